@@ -1,0 +1,210 @@
+// window_attn.hip -- attention with a sliding window and visible first tokens: forward pass (gfx950).  The rule of visibility and the fragment layout are in
+// window_attn_device.h, the backward pass in window_attn_bwd.hip, the single-token form in window_attn_step.hip.
+//
+//   s_ij = scale q_i . k_j over the visible keys,  p_ij = exp(s_ij - m_i) / l_i,  o_i = sum_j p_ij v_j,   m the running maximum, l the running sum (fp32)
+//
+// A workgroup takes 128 queries of one head, a wavefront 32 of them, and walks the tiles of keys that they can see (the sinks' tiles, then the band's): keys and
+// values go through LDS, double-buffered, the tile after next in flight in registers, one barrier per tile.  S^T = K Q^T puts a query's scores into ONE lane pair: the
+// row maximum and sum are register arithmetic, the probabilities are the operand of O^T = V^T P^T without leaving their registers, and the accumulators are rescaled
+// by one factor per lane -- only when a maximum has grown by more than 2^8, since exp2(s - m) with a slightly old m is as exact.
+// Probabilities are rounded to the operand type (16-bit modes) for the matrix instruction; l sums the unrounded ones in fp32.
+#include "window_attn_device.h"
+
+namespace gfpp {
+
+template <typename T, int DP>
+constexpr int wa_bn() { return sizeof(T) == 4 && DP == 128 ? 32 : 64; }
+
+template <typename T, int DP, bool VEC>
+__global__ __launch_bounds__(kWaThreads, sizeof(T) == 2 ? 2 : 1) void k_window_attn(WaArgs a) {
+    constexpr int BN = wa_bn<T, DP>(), NS = DP / 16, NT = DP / 32, NSUB = BN / 32, PK = wa_pitch_row<T, DP>(), PV = wa_pitch_col<T, DP>();
+    typedef typename LpTraits<T>::vec vec;
+    __shared__ __attribute__((aligned(16))) unsigned char s_k[2][BN * PK], s_v[2][BN * PV];
+    const int q_tiles = (a.Tq + kWaRows - 1) / kWaRows;
+    const int hq = (int)(blockIdx.x / q_tiles) % a.Hq, b = (int)(blockIdx.x / q_tiles) / a.Hq, i0 = (int)(blockIdx.x % q_tiles) * kWaRows, hk = hq / a.G;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = lane & 31, h = lane >> 5;
+    const int n = a.lengths ? a.lengths[b] < a.Tk ? a.lengths[b] : a.Tk : a.Tk;
+    const int i = i0 + wave * 32 + c, p = a.q_start + i;
+    const bool have = i < a.Tq && p < n;
+    vec q[NS];
+    wa_global_rows<T, NS, VEC>(q, static_cast<const T *>(a.q.p) + b * a.q.sb + (int64_t)i * a.q.st + hq * a.q.sh, have, h, a.D);
+    const int i1 = i0 + kWaRows < a.Tq ? i0 + kWaRows - 1 : a.Tq - 1;
+    const WaRange range = wa_keys<BN>(a, a.q_start + i0, a.q_start + i1, n);
+    const int tiles = range.head + range.hi - range.lo;
+    const int last = have ? (p + a.right < n - 1 ? p + a.right : n - 1) : -1, first = p - a.left;          // this lane's query
+    const int pw0 = a.q_start + i0 + wave * 32, pw1 = pw0 + 31;                                               // the wavefront's
+    v16f acc[NT];
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) acc[t][r] = 0.0f;
+    float m = -INFINITY, l = 0.0f;
+    const T *kb = static_cast<const T *>(a.k.p) + b * a.k.sb + hk * a.k.sh, *vb = static_cast<const T *>(a.v.p) + b * a.v.sb + hk * a.v.sh;
+    WaStage<T, DP, BN, VEC> rk, rv;
+    auto tile_row = [&](int k) { return (k < range.head ? k : range.lo + k - range.head) * BN; };
+    if (tiles > 0) {
+        rk.load(kb, a.k.st, tile_row(0), n, a.D);
+        rv.load(vb, a.v.st, tile_row(0), n, a.D);
+        rk.store(s_k[0], PK);
+        rv.store(s_v[0], PV);
+        if (tiles > 1) {
+            rk.load(kb, a.k.st, tile_row(1), n, a.D);
+            rv.load(vb, a.v.st, tile_row(1), n, a.D);
+        }
+    }
+    __syncthreads();
+    const int row_at = c * PK + 8 * h * (int)sizeof(T), col_at = wa_col_offset<T>(lane, PV);
+    for (int k = 0; k < tiles; ++k) {
+        const int buf = k & 1, j0 = tile_row(k), j1 = j0 + BN - 1;
+        if (k + 1 < tiles) {
+            rk.store(s_k[buf ^ 1], PK);                     // (last read before the previous barrier)
+            rv.store(s_v[buf ^ 1], PV);
+            if (k + 2 < tiles) {
+                rk.load(kb, a.k.st, tile_row(k + 2), n, a.D);
+                rv.load(vb, a.v.st, tile_row(k + 2), n, a.D);
+            }
+        }
+        const bool seen = pw0 < n && j0 <= pw1 + a.right && (j1 >= pw0 - a.left || j0 < a.sinks);
+        if (seen) {
+            v16f s[NSUB];
+#pragma unroll
+            for (int u = 0; u < NSUB; ++u) {
+#pragma unroll
+                for (int r = 0; r < 16; ++r) s[u][r] = 0.0f;
+#pragma unroll
+                for (int x = 0; x < NS; ++x) s[u] = LpTraits<T>::mfma(wa_row<T>(s_k[buf] + row_at + 32 * u * PK, x), q[x], s[u]);
+            }
+            const bool full = pw1 < n && j1 < n && j1 <= pw0 + a.right && (j0 >= pw1 - a.left || j1 < a.sinks);
+            if (!full) {
+#pragma unroll
+                for (int u = 0; u < NSUB; ++u)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) {
+                        const int j = j0 + 32 * u + 8 * (r >> 2) + 4 * h + (r & 3);
+                        s[u][r] = j <= last && (j >= first || j < a.sinks) ? s[u][r] : -INFINITY;
+                    }
+            }
+            float top = s[0][0];
+#pragma unroll
+            for (int u = 0; u < NSUB; ++u)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) top = fmaxf(top, s[u][r]);
+            top = half_wave_max(top);
+            // (both -inf: NaN, which is not > 8; the first visible score: inf > 8)
+            if (__any((top - m) * a.c > 8.0f)) {
+                const float grown = fmaxf(m, top), f = m == -INFINITY ? 0.0f : exp2f((m - grown) * a.c);
+                m = grown;
+                l *= f;
+#pragma unroll
+                for (int t = 0; t < NT; ++t)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) acc[t][r] *= f;
+            }
+            const float top0 = m == -INFINITY ? 0.0f : m, base = top0 * a.c;
+#pragma unroll
+            for (int u = 0; u < NSUB; ++u)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    s[u][r] = wa_prob<T>(s[u][r], top0, base, a.c);
+                    l += s[u][r];
+                }
+#pragma unroll
+            for (int u = 0; u < NSUB; ++u)
+#pragma unroll
+                for (int x = 0; x < 2; ++x) {
+                    const vec pr = wa_pack<T>(s[u], x);
+#pragma unroll
+                    for (int t = 0; t < NT; ++t) acc[t] = LpTraits<T>::mfma(wa_col<T, PV>(s_v[buf] + col_at, 32 * u + 16 * x, t), pr, acc[t]);
+                }
+        }
+        __syncthreads();
+    }
+    l = half_wave_sum(l);
+    if (i >= a.Tq) return;
+    T *o = static_cast<T *>(a.o.p) + b * a.o.sb + (int64_t)i * a.o.st + hq * a.o.sh;
+    wa_store_rows<T, NT, VEC>(acc, l > 0.0f ? 1.0f / l : 0.0f, o, h, a.D);
+    // log2 of the row's sum, +inf for a row without visible keys: every probability of the backward pass is then exp2(-inf) = 0
+    if (a.lse && h == 0) a.lse[((int64_t)b * a.Hq + hq) * a.Tq + i] = l > 0.0f ? m * a.c + log2f(l) : INFINITY;
+}
+
+bool wa_vectors(const WaTensor &t, int D, size_t size) {
+    return ((uintptr_t)t.p | (uint64_t)(t.sb * (int64_t)size) | (uint64_t)(t.st * (int64_t)size) | (uint64_t)(t.sh * (int64_t)size) | (uint64_t)(D * size)) % 16 == 0;
+}
+
+// the arguments that both passes share; 0 or an error code
+int wa_arguments(const char *what, WaArgs &a, const int64_t *strides, int n_tensors, uint32_t B, uint32_t Tq, uint32_t Tk, uint32_t Hq, uint32_t Hk, uint32_t D, int32_t left,
+                 int32_t right, int32_t sinks, int32_t q_start, const int32_t *lengths, float scale, int dtype) {
+    const uint32_t most = 1u << 29;
+#define WA_REQUIRE(cond)                                               \
+    do {                                                               \
+        if (!(cond)) {                                                 \
+            set_error("%s: invalid argument (%s)", what, #cond);       \
+            return GFPP_EINVAL;                                        \
+        }                                                              \
+    } while (0)
+    WA_REQUIRE(dtype == GFPP_F32 || dtype == GFPP_F16 || dtype == GFPP_BF16);
+    WA_REQUIRE(B <= most && Tq <= most && Tk <= most && Hq <= most && Hk <= most && strides);
+    WA_REQUIRE(Hk >= 1 && Hq >= 1 && Hq % Hk == 0);
+    WA_REQUIRE(left >= 0 && right >= 0 && sinks >= 0 && q_start >= 0 && (uint32_t)q_start <= most);
+    WA_REQUIRE(scale > 0.0f && scale < INFINITY);
+    if (D < 1 || D > 128) {
+        set_error("%s: head width %u (1 .. 128 are supported)", what, D);
+        return GFPP_EUNSUPPORTED;
+    }
+    WaTensor *t[8] = {&a.q, &a.k, &a.v, &a.o, &a.dout, &a.dq, &a.dk, &a.dv};
+    for (int k = 0; k < n_tensors; ++k) {
+        t[k]->sb = strides[3 * k];
+        t[k]->st = strides[3 * k + 1];
+        t[k]->sh = strides[3 * k + 2];
+    }
+    a.lengths = lengths;
+    a.B = (int)B;
+    a.Tq = (int)Tq;
+    a.Tk = (int)Tk;
+    a.Hq = (int)Hq;
+    a.Hk = (int)Hk;
+    a.G = (int)(Hq / Hk);
+    a.D = (int)D;
+    a.left = left < (int)most ? left : (int)most;
+    a.right = right < (int)most ? right : (int)most;
+    a.sinks = sinks < (int)Tk ? sinks : (int)Tk;
+    a.q_start = q_start;
+    a.scale = scale;
+    a.c = scale * 1.4426950408889634f;
+    return 0;
+}
+
+template <typename T>
+static void wa_forward(const WaArgs &a, bool vec, uint32_t grid, hipStream_t st) {
+    if (a.D <= 32) vec ? k_window_attn<T, 32, true><<<grid, kWaThreads, 0, st>>>(a) : k_window_attn<T, 32, false><<<grid, kWaThreads, 0, st>>>(a);
+    else if (a.D <= 64) vec ? k_window_attn<T, 64, true><<<grid, kWaThreads, 0, st>>>(a) : k_window_attn<T, 64, false><<<grid, kWaThreads, 0, st>>>(a);
+    else vec ? k_window_attn<T, 128, true><<<grid, kWaThreads, 0, st>>>(a) : k_window_attn<T, 128, false><<<grid, kWaThreads, 0, st>>>(a);
+}
+
+}  // namespace gfpp
+
+using namespace gfpp;
+
+GFPP_API int gfpp_window_attn_forward(const void *q, const void *k, const void *v, void *out, float *lse, const int64_t *strides, uint32_t B, uint32_t Tq, uint32_t Tk,
+                                      uint32_t Hq, uint32_t Hk, uint32_t D, int32_t left, int32_t right, int32_t sinks, int32_t q_start, const int32_t *lengths, float scale,
+                                      int dtype, gfpp_stream_t stream) {
+    const char *what = "gfpp_window_attn_forward";
+    WaArgs a{};
+    if (int rc = wa_arguments(what, a, strides, 4, B, Tq, Tk, Hq, Hk, D, left, right, sinks, q_start, lengths, scale, dtype)) return rc;
+    if ((uint64_t)B * Tq == 0) return 0;
+    WA_REQUIRE(q && out && (Tk == 0 || (k && v)));
+    a.q.p = const_cast<void *>(q);
+    a.k.p = const_cast<void *>(k);
+    a.v.p = const_cast<void *>(v);
+    a.o.p = out;
+    a.lse = lse;
+    const uint64_t grid = (uint64_t)div_up(Tq, kWaRows) * Hq * B;
+    WA_REQUIRE(grid <= 0x7fffffffull);
+    const size_t size = dtype == GFPP_F32 ? 4 : 2;
+    const bool vec = wa_vectors(a.q, a.D, size) && wa_vectors(a.k, a.D, size) && wa_vectors(a.v, a.D, size) && wa_vectors(a.o, a.D, size);
+    hipStream_t st = (hipStream_t)stream;
+    if (dtype == GFPP_F32) wa_forward<float>(a, vec, (uint32_t)grid, st);
+    else if (dtype == GFPP_F16) wa_forward<_Float16>(a, vec, (uint32_t)grid, st);
+    else wa_forward<__bf16>(a, vec, (uint32_t)grid, st);
+    return check_launch(what);
+}

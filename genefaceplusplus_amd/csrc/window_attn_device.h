@@ -1,0 +1,255 @@
+// window_attn_device.h -- what the windowed-attention kernels share (window_attn.hip, window_attn_bwd.hip; gfx950).
+//
+// A query at position p = q_start + i sees key j iff  j < n  and  p < n  and  j <= p + right  and  (j >= p - left  or  j < sinks),  n = the sequence's length.
+//
+// Fragments of v_mfma_f32_32x32x16_*: lane (c = lane & 31, h = lane >> 5) supplies row / column c at contraction indices 8 h .. 8 h + 7 of a step, and holds of a
+// 32 x 32 product column c at rows  8 (r >> 2) + 4 h + (r & 3), r = 0 .. 15.  The contraction index may be permuted as long as both operands agree, so the 16
+// values of a product that a lane holds ARE the operand of the next product's two steps (values 8 s .. 8 s + 7 = rows 16 s + {4 h .. 4 h + 3, 8 + 4 h .. 8 + 4 h + 3}):
+// probabilities never leave their registers, the other operand is read with the rows in that order.  fp32: a "step" is eight v_mfma_f32_32x32x2_f32, element e of
+// both fragments each (lp_mfma_device.h).
+#pragma once
+
+#include "gfpp_common.h"
+#include "lp_mfma_device.h"
+
+namespace gfpp {
+
+constexpr int kWaThreads = 256, kWaRows = 128;      // four wavefronts of 32 queries (forward, dq) or 32 keys (dk, dv)
+
+struct WaTensor {
+    void *p;
+    int64_t sb, st, sh;            // strides of sequence, token and head in elements
+};
+struct WaArgs {
+    WaTensor q, k, v, o, dout, dq, dk, dv;
+    float *lse, *delta;            // [B][Hq][Tq]
+    float *partial;                // sink tiles' dk and dv: [sink tiles][splits][B][Hk][2][128][D]
+    const int32_t *lengths;        // [B] or NULL
+    int32_t B, Tq, Tk, Hq, Hk, D, G;
+    int32_t left, right, sinks;    // left, right < 2^30
+    int32_t q_start;
+    float scale, c;                // c = scale log2(e)
+    uint32_t sink_tiles, splits;
+};
+
+template <typename T>
+struct WaTraits;
+template <>
+struct WaTraits<_Float16> {
+    static constexpr int V = 8;                                        // elements of 16 bytes
+    typedef __fp16 raw4 __attribute__((__vector_size__(8)));
+    typedef _Float16 half4 __attribute__((ext_vector_type(4)));
+};
+template <>
+struct WaTraits<__bf16> {
+    static constexpr int V = 8;
+    typedef __bf16 half4 __attribute__((ext_vector_type(4)));
+};
+template <>
+struct WaTraits<float> {
+    static constexpr int V = 4;
+};
+
+// Bytes of an LDS row of DP elements, padded for what reads it (64 banks of 4 bytes): row fragments want an odd number of 16-byte units (16 rows at one column
+// then cover all banks), transposing reads 64 or 192 modulo 256 bytes (the 4 rows x 64 bytes of one read lie apart); rows that are read both ways take the odd
+// number next to that.  32-bit columns are read a word per lane: any pitch.
+template <typename T, int DP>
+constexpr int wa_pitch_row() { return DP * (int)sizeof(T) + 16; }
+template <typename T, int DP>
+constexpr int wa_pitch_col() { return DP * (int)sizeof(T) % 128 == 0 ? DP * (int)sizeof(T) + 64 : DP * (int)sizeof(T); }
+template <typename T, int DP>
+constexpr int wa_pitch_both() { return DP * (int)sizeof(T) + (sizeof(T) == 2 ? (DP == 32 ? 16 : 80) : 16); }
+
+// rows r0 .. r0 + ROWS - 1 of a [tokens][D] head into registers, the thread's share: 16 bytes per vector.  Rows from `end` on and columns from D on are zeros and
+// are not read: what lies behind a sequence may hold anything.
+template <typename T, int DP, int ROWS, bool VEC>
+struct WaStage {
+    static constexpr int V = WaTraits<T>::V, PER_ROW = DP / V, N = ROWS * PER_ROW / kWaThreads;
+    static_assert(ROWS * PER_ROW % kWaThreads == 0, "whole vectors per thread");
+    typedef T vec __attribute__((ext_vector_type(V)));
+    vec r[N];
+
+    __device__ __forceinline__ void load(const T *base, int64_t stride, int r0, int end, int D) {
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+            const int i = n * kWaThreads + (int)threadIdx.x, row = r0 + i / PER_ROW, col = i % PER_ROW * V;
+            vec t = (vec)(T)0.0f;
+            if (row < end && row >= 0 && col < D) {
+                const T *p = base + (int64_t)row * stride + col;
+                if constexpr (VEC) {
+                    t = *reinterpret_cast<const vec *>(p);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < V; ++e)
+                        if (col + e < D) t[e] = p[e];
+                }
+            }
+            r[n] = t;
+        }
+    }
+    __device__ __forceinline__ void store(unsigned char *lds, int pitch) const {
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+            const int i = n * kWaThreads + (int)threadIdx.x;
+            *reinterpret_cast<vec *>(lds + i / PER_ROW * pitch + i % PER_ROW * 16) = r[n];
+        }
+    }
+};
+
+// row fragment: elements 16 s + 8 h .. + 7 of row c of a tile (`at` = the lane's row + 8 h elements)
+template <typename T>
+__device__ __forceinline__ typename LpTraits<T>::vec wa_row(const unsigned char *at, int s) {
+    return *reinterpret_cast<const typename LpTraits<T>::vec *>(at + s * 16 * (int)sizeof(T));
+}
+template <>
+__device__ __forceinline__ LpTraits<float>::vec wa_row<float>(const unsigned char *at, int s) {
+    typedef float f4 __attribute__((ext_vector_type(4)));
+    const f4 a = *reinterpret_cast<const f4 *>(at + s * 64), b = *reinterpret_cast<const f4 *>(at + s * 64 + 16);
+    return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+}
+
+// column fragment of the 16 rows from row0 (tile bytes `tile`): column 32 t + c at rows {4 h .. 4 h + 3, 8 + 4 h .. 8 + 4 h + 3}.  16 bits: two transposing reads
+// (ds_read_b64_tr_b16: a quarter wavefront reads 4 rows x 16 columns, lane p the four elements at its own address -- row p >> 2, columns 4 (p & 3) .. -- and lane l
+// is given column l); 32 bits: eight reads.
+template <typename T>
+__device__ __forceinline__ int wa_col_offset(int lane, int pitch) {
+    const int c = lane & 31, h = lane >> 5;
+    if constexpr (sizeof(T) == 4) return 4 * h * pitch + c * 4;
+    const int p = lane & 15, gi = (lane >> 4) & 1;
+    return (4 * h + (p >> 2)) * pitch + (16 * gi + 4 * (p & 3)) * 2;
+}
+template <typename T, int PITCH>
+__device__ __forceinline__ typename LpTraits<T>::vec wa_col(const unsigned char *tile_at, int row0, int t) {
+    const unsigned char *at = tile_at + row0 * PITCH + t * 32 * (int)sizeof(T);
+    if constexpr (sizeof(T) == 4) {
+        typename LpTraits<T>::vec f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) f[e] = *reinterpret_cast<const float *>(at + ((e & 3) + 8 * (e >> 2)) * PITCH);
+        return f;
+    } else {
+        typedef __attribute__((__vector_size__(4 * sizeof(__fp16)))) __fp16 fp16x4;
+        typedef __attribute__((address_space(3))) fp16x4 *lds_ptr;
+        typedef T half4 __attribute__((ext_vector_type(4)));
+        const fp16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4f16((lds_ptr)(at));
+        const fp16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4f16((lds_ptr)(at + 8 * PITCH));
+        return __builtin_shufflevector(__builtin_bit_cast(half4, lo), __builtin_bit_cast(half4, hi), 0, 1, 2, 3, 4, 5, 6, 7);
+    }
+}
+
+// the lane's row of a head straight from memory as NS row fragments; zeros where `have` is false and behind column D
+template <typename T, int NS, bool VEC>
+__device__ __forceinline__ void wa_global_rows(typename LpTraits<T>::vec (&f)[NS], const T *row, bool have, int h, int D) {
+    typedef T vec16 __attribute__((ext_vector_type(WaTraits<T>::V)));
+#pragma unroll
+    for (int s = 0; s < NS; ++s) {
+        const int col = 16 * s + 8 * h;
+#pragma unroll
+        for (int e0 = 0; e0 < 8; e0 += WaTraits<T>::V) {
+            vec16 t = (vec16)(T)0.0f;
+            if (have && col + e0 < D) {
+                if constexpr (VEC) {
+                    t = *reinterpret_cast<const vec16 *>(row + col + e0);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < WaTraits<T>::V; ++e)
+                        if (col + e0 + e < D) t[e] = row[col + e0 + e];
+                }
+            }
+#pragma unroll
+            for (int e = 0; e < WaTraits<T>::V; ++e) f[s][e0 + e] = t[e];
+        }
+    }
+}
+
+// values 8 s .. 8 s + 7 of a product, rounded to the operand type (pairs: one conversion instruction each)
+template <typename T>
+__device__ __forceinline__ typename LpTraits<T>::vec wa_pack(const v16f &x, int s) {
+    if constexpr (sizeof(T) == 4) {
+        typename LpTraits<T>::vec f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) f[e] = x[8 * s + e];
+        return f;
+    } else {
+        typedef float f32x2 __attribute__((ext_vector_type(2)));
+        typename LpTraits<T>::vec f;
+#pragma unroll
+        for (int e = 0; e < 8; e += 2) {
+            const typename LpTraits<T>::pair p = __builtin_convertvector(((f32x2){x[8 * s + e], x[8 * s + e + 1]}), typename LpTraits<T>::pair);
+            f[e] = p[0];
+            f[e + 1] = p[1];
+        }
+        return f;
+    }
+}
+
+// exp2((s - m) c), base = m c.  16-bit modes: one fused multiply-add; its rounding of base is far below theirs.  fp32: the difference first, so that the largest
+// score's probability is exactly 1 and a query with one visible key copies its value
+template <typename T>
+__device__ __forceinline__ float wa_prob(float s, float m, float base, float c) {
+    if constexpr (sizeof(T) == 4) return __builtin_amdgcn_exp2f((s - m) * c);
+    return __builtin_amdgcn_exp2f(fmaf(s, c, -base));
+}
+
+__device__ __forceinline__ float half_wave_max(float t) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(t), __float_as_uint(t), false, false);
+    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+
+// x f rounded to 32 bits and then to T in every form of the kernels: left alone, the compiler makes some scalar f16 stores a mixed-precision multiply that rounds once
+template <typename T>
+__device__ __forceinline__ T wa_scaled(float x, float f) {
+    float y = x * f;
+    asm("" : "+v"(y));
+    return (T)y;
+}
+
+// a product tile [32 T rows = features][32 columns = tokens] to the lane's token row: 4 consecutive features per store
+template <typename T, int NT, bool VEC>
+__device__ __forceinline__ void wa_store_rows(const v16f (&acc)[NT], float f, T *row, int h, int D) {
+    typedef T vec4 __attribute__((ext_vector_type(4)));
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int r = 0; r < 16; r += 4) {
+            const int col = 32 * t + 2 * r + 4 * h;
+            if (col >= D) continue;
+            if (VEC || col + 3 < D) {
+                vec4 v;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v[e] = wa_scaled<T>(acc[t][r + e], f);
+                if constexpr (VEC) {
+                    *reinterpret_cast<vec4 *>(row + col) = v;
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) row[col + e] = v[e];
+                }
+            } else {
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (col + e < D) row[col + e] = wa_scaled<T>(acc[t][r + e], f);
+            }
+        }
+}
+
+// tiles of BN keys that queries at positions p0 .. p1 can see: [0, head) for the sinks in front of the band, [lo, hi) for the band (merged where they touch)
+struct WaRange {
+    int head, lo, hi;
+};
+template <int BN>
+__device__ __forceinline__ WaRange wa_keys(const WaArgs &a, int p0, int p1, int n) {
+    WaRange r{0, 0, 0};
+    if (p1 >= n) p1 = n - 1;
+    if (p0 > p1) return r;
+    const int last = p1 + a.right < n - 1 ? p1 + a.right : n - 1, first = p0 - a.left > 0 ? p0 - a.left : 0;
+    r.lo = first / BN;
+    r.hi = last / BN + 1;
+    const int s = a.sinks < n ? a.sinks : n;
+    r.head = (s + BN - 1) / BN;
+    if (r.head >= r.lo) {
+        r.lo = 0;
+        r.head = 0;
+    }
+    return r;
+}
+
+}  // namespace gfpp

@@ -2,7 +2,8 @@
 from .head import NeRFRenderer, RADNeRF
 from .torso import RADNeRFTorso, RADNeRFTorsowithSR, RADNeRFwithSR
 from .cond_nets import AudioNet, AudioAttNet, MLP
-from .encoders import GridEncoder, SHEncoder, FreqEncoder, get_encoder
+from .encoders import GridEncoder, SHEncoder, FreqEncoder, RotaryEncoder, get_encoder, rotary_embed
+from .sequence import LayerNorm, WindowCache, layer_norm, window_attention, window_attention_step
 from ..configs import CLASSES
 
 _RUNTIME_HPARAMS = {}

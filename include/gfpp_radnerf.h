@@ -843,6 +843,60 @@ typedef struct gfpp_sr_ws { /* caller-allocated device workspace */
 int gfpp_sr_forward(const gfpp_sr_model *model, const gfpp_sr_ws *ws, const float *rgb_in, const float *const noise[4], float *rgb_out,
                     gfpp_stream_t stream);
 
+/* ------------------------------------------------------------------------------------------------------------
+ * Section C -- sequence operators of the conditioning stage (beside AudioNet / AudioAttNet, cond_encoder.py:98-180, which smooth windows of 1 .. 16 frames; the
+ * reference has no native counterpart).  dtype: GFPP_F32 / GFPP_F16 / GFPP_BF16, the type of every tensor that is not named otherwise; statistics, softmax sums
+ * and reductions are fp32.  Strides are in elements; the last axis of every tensor has stride 1; rows may start anywhere (16-byte vectors where every pointer and
+ * stride allows them, single elements otherwise).  `strides`, `sections` are HOST arrays.  Scratch is the caller's, per call; nothing is kept between calls.
+ * ---------------------------------------------------------------------------------------------------------- */
+
+/* Layer norm over the last axis in front of a conditioning network's layers (cond_encoder.py:98-143 has none): y[m] = (x[m] - mean) / sqrt(var + eps) * weight +
+ * bias for M rows of N, x's rows x_pitch apart, y contiguous.  weight, bias [N] of param_dtype (GFPP_F32 or dtype) or NULL.  mean, rstd [M] f32: both (for the backward pass)
+ * or NULL. */
+int gfpp_layer_norm_forward(const void *x, int64_t x_pitch, const void *weight, const void *bias, int param_dtype, uint64_t M, uint32_t N, float eps, int dtype,
+                            void *y, float *mean, float *rstd, gfpp_stream_t stream);
+/* Its backward pass (cond_encoder.py:98-143, as above): dx [M, N] contiguous, dweight and dbias [N] of param_dtype, each may be NULL; scratch: as many floats as
+ * gfpp_layer_norm_backward_scratch_floats says, for dweight / dbias only.  Sums in a fixed order. */
+int gfpp_layer_norm_backward(const void *dy, int64_t dy_pitch, const void *x, int64_t x_pitch, const void *weight, int param_dtype, const float *mean,
+                             const float *rstd, uint64_t M, uint32_t N, int dtype, void *dx, void *dweight, void *dbias, float *scratch, gfpp_stream_t stream);
+/* (cond_encoder.py:98-143, as above) */
+unsigned long long gfpp_layer_norm_backward_scratch_floats(uint64_t M, uint32_t N);
+
+/* Rotary positions over 1 .. 4 axes, beside the frequency encoding of coordinates (encoders/encoding.py:6-35): x0 [B, T, heads0, D] -> y0 (contiguous), and x1 -> y1
+ * in the same launch (heads1 = 0: none).  x_strides: {B, T, heads}.  The first 2 P features of a head, P = sections[0] + ... + sections[axes - 1], are P pairs --
+ * (i, i + P), or (2 i, 2 i + 1) when interleaved -- turned by position[axis of i] * frequencies[i] radians; the rest passes through.  positions: [B, T, axes]
+ * int32 (position_type 0), int64 (1) or f32 (2), position_stride between sequences (0: one set for all); frequencies [P] f64.  backward: turned the other way. */
+int gfpp_rotary(const void *x0, const int64_t *x0_strides, uint32_t heads0, void *y0, const void *x1, const int64_t *x1_strides, uint32_t heads1, void *y1,
+                const void *positions, int position_type, int64_t position_stride, const double *frequencies, const uint32_t *sections, uint32_t axes, uint32_t B,
+                uint32_t T, uint32_t D, int interleaved, int backward, int dtype, gfpp_stream_t stream);
+
+/* Attention with a sliding window and visible first tokens over a conditioning sequence (AudioAttNet's weighted window, cond_encoder.py:146-180, for sequences of any
+ * length): out[b, i, h] = sum_j softmax_j(scale q[b, i, h] . k[b, j, h / G]) v[b, j, h / G], G = Hq / Hk, over the keys j that the query at position p = q_start + i
+ * sees:  j < n and p < n and j <= p + right and (j >= p - left or j < sinks),  n = min(lengths[b], Tk) (lengths NULL: Tk).  A query that sees nothing gives
+ * zeros.  q, out [B, Tq, Hq, D]; k, v [B, Tk, Hk, D]; strides: {B, T, H} of q, k, v, out; D 1 .. 128.  lse [B, Hq, Tq] f32 for the backward pass, or NULL.
+ * Rows behind a sequence's length are not read (they may hold anything); within it keys and values have to be finite. */
+int gfpp_window_attn_forward(const void *q, const void *k, const void *v, void *out, float *lse, const int64_t *strides, uint32_t B, uint32_t Tq, uint32_t Tk,
+                             uint32_t Hq, uint32_t Hk, uint32_t D, int32_t left, int32_t right, int32_t sinks, int32_t q_start, const int32_t *lengths, float scale,
+                             int dtype, gfpp_stream_t stream);
+/* Its backward pass (cond_encoder.py:146-180, as above): dq, dk, dv from dout, the forward pass' inputs, out and lse.  strides: {B, T, H} of q, k, v, out, dout, dq,
+ * dk, dv.  Every row of dq, dk and dv is written (zeros behind a sequence's length).  No atomics: the same bits every time. */
+int gfpp_window_attn_backward(const void *q, const void *k, const void *v, const void *out, const void *dout, const float *lse, void *dq, void *dk, void *dv,
+                              float *scratch, const int64_t *strides, uint32_t B, uint32_t Tq, uint32_t Tk, uint32_t Hq, uint32_t Hk, uint32_t D, int32_t left,
+                              int32_t right, int32_t sinks, int32_t q_start, const int32_t *lengths, float scale, int dtype, gfpp_stream_t stream);
+/* (cond_encoder.py:146-180, as above) */
+unsigned long long gfpp_window_attn_backward_scratch_floats(uint32_t B, uint32_t Tq, uint32_t Tk, uint32_t Hq, uint32_t Hk, uint32_t D, int32_t left,
+                                                            int32_t sinks, int32_t q_start);
+
+/* One new token per stream (AudioAttNet's weighted window, cond_encoder.py:146-180, for a live stream): stream b's token at positions[b] (int32, or int64 with
+ * positions64) writes k[b], v[b] [Hk, D] into its slot of cache_k, cache_v [B, slots, Hk, D] -- n < sinks ? n : sinks + (n - sinks) mod (slots - sinks) -- and
+ * out[b] [Hq, D] is its attention over the min(n + 1, slots) filled slots: gfpp_window_attn_forward's row n with left = slots - sinks - 1, right = 0.  A negative
+ * position: the stream is left as it is and its output is zeros.  strides: q {B, H}, k {B, H}, v {B, H}, cache_k {B, slot, H}, cache_v {B, slot, H}, out {B, H}. */
+int gfpp_window_attn_step(const void *q, const void *k, const void *v, void *cache_k, void *cache_v, const void *positions, int positions64, void *out,
+                          const int64_t *strides, uint32_t B, uint32_t Hq, uint32_t Hk, uint32_t D, uint32_t slots, uint32_t sinks, float scale, int dtype,
+                          float *scratch, gfpp_stream_t stream);
+/* (cond_encoder.py:146-180, as above) */
+unsigned long long gfpp_window_attn_step_scratch_floats(uint32_t B, uint32_t Hq, uint32_t Hk, uint32_t D, uint32_t slots);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,185 @@
+"""What the sequence operators refuse, without a GPU: the Python entry points (their launch replaced) and the C entry points, which check before they launch anything."""
+import ctypes
+
+import pytest
+import torch
+
+from genefaceplusplus_amd import _lib
+from genefaceplusplus_amd._lib import GfppError
+from genefaceplusplus_amd.radnerfs import RotaryEncoder, WindowCache, encoders, get_encoder, layer_norm, rotary_embed, sequence, window_attention, window_attention_step
+
+bf16, f16, f32, f64 = torch.bfloat16, torch.float16, torch.float32, torch.float64
+
+
+class Launched(Exception):
+    pass
+
+
+@pytest.fixture
+def no_launch(monkeypatch):
+    """CPU tensors pass for the GPU's, a launch raises Launched with its entry point."""
+    def stop(device, name, *args):
+        raise Launched(name)
+    real = sequence.check_tensors
+
+    def check(what, like, **tensors):
+        class Like:
+            is_cuda, dtype, device = True, like.dtype, like.device
+        real(what, Like, **tensors)
+    for module in (sequence, encoders):
+        monkeypatch.setattr(module, "launch", stop)
+        monkeypatch.setattr(module, "check_tensors", check)
+    monkeypatch.setattr(sequence, "scratch_floats", lambda *a: 0)
+
+
+def z(*shape, dtype=f32):
+    return torch.zeros(*shape, dtype=dtype)
+
+
+def test_no_cpu_path():
+    q = z(1, 4, 2, 8)
+    for call in (lambda: layer_norm(z(3, 8)), lambda: window_attention(q, q, q), lambda: window_attention_step(q[:, 0], q[:, 0], q[:, 0], q, q, z(1, dtype=torch.int32)),
+                 lambda: RotaryEncoder(8, (4,))(q, torch.zeros(4, 1))):
+        with pytest.raises(GfppError, match="must be on the GPU"):
+            call()
+
+
+def test_layer_norm_refusals(no_launch):
+    x = z(3, 8)
+    with pytest.raises(Launched, match="gfpp_layer_norm_forward"):
+        layer_norm(x, z(8), z(8))
+    for args, why in (((z(3, 8, dtype=f64),), "float32, float16 or bfloat16"), ((x, z(7)), "weight must be"), ((x, None, z(8, 1)), "bias must be"), ((x, z(16)[::2]), "weight must be"),
+                      ((x, z(8, dtype=f16)), "weight must be float32"), ((z(3, 8, dtype=bf16), z(8), z(8, dtype=bf16)), "weight is"), ((z(3, 0),), "last axis"),
+                      ((z(()),), "last axis"), ((x, None, None, -1.0), "eps"), ((x, None, None, float("nan")), "eps")):
+        with pytest.raises(GfppError, match=why):
+            layer_norm(*args)
+
+
+def test_rotary_refusals(no_launch):
+    x, p, f = z(2, 3, 4, 16), z(3, 2), z(8, dtype=f64)
+    ok = dict(x=x, positions=p, frequencies=f, sections=(3, 5))
+    with pytest.raises(Launched, match="gfpp_rotary"):
+        rotary_embed(**ok)
+    for change, why in ((dict(x=z(3, 4, 16)), "tensors of one type"), (dict(x=(x, z(2, 3, 1, 8))), "tensors of one type"), (dict(x=(x, x.half())), "tensors of one type"),
+                        (dict(x=(x, x, x)), "one tensor or two"), (dict(sections=(3, 6), frequencies=z(9, dtype=f64)), "sections"), (dict(sections=()), "sections"),
+                        (dict(sections=(-1, 9)), "sections"), (dict(sections=(1, 1, 1, 1, 4)), "sections"), (dict(positions=z(3, 2, dtype=f64)), "positions"),
+                        (dict(positions=z(3)), "positions"), (dict(positions=z(1, 3, 2)), "positions"), (dict(frequencies=z(8)), "frequencies"),
+                        (dict(frequencies=z(7, dtype=f64)), "frequencies"), (dict(x=x.double()), "float32, float16 or bfloat16")):
+        with pytest.raises(GfppError, match=why):
+            rotary_embed(**{**ok, **change})
+    with pytest.raises(GfppError, match="sections"):
+        RotaryEncoder(8, (5,))
+    with pytest.raises(GfppError, match="built for heads"):
+        get_encoder("rotary", input_dim=1, dim=32)[0](x, z(3, 1))
+
+
+def test_attention_refusals(no_launch):
+    q, k = z(2, 5, 4, 16), z(2, 9, 2, 16)
+    with pytest.raises(Launched, match="gfpp_window_attn_forward"):
+        window_attention(q, k, k)
+    n = lambda *v, dtype=torch.int32: torch.tensor(v, dtype=dtype)  # noqa: E731
+    for args, how, why in (((q, k, k.half()), {}, "one type"), ((q[0], k, k), {}, "axes"), ((q, k, k[:, :8]), {}, "shape of v"), ((q[:1], k, k), {}, "batch or head width"),
+                           ((q, k[..., :8], k[..., :8]), {}, "batch or head width"), ((z(2, 5, 3, 16), k, k), {}, "multiple"), ((z(2, 5, 0, 16), k, k), {}, "multiple"),
+                           ((z(2, 5, 4, 129), z(2, 5, 4, 129), z(2, 5, 4, 129)), {}, "head width 129"), ((z(2, 5, 4, 0), z(2, 5, 4, 0), z(2, 5, 4, 0)), {}, "head width 0"),
+                           ((q, k, k), dict(left=-1), "left"), ((q, k, k), dict(right=-2), "right"), ((q, k, k), dict(right=1.5), "right"), ((q, k, k), dict(sinks=-1), "sinks"),
+                           ((q, k, k), dict(scale=0.0), "scale"), ((q, k, k), dict(scale=-1.0), "scale"), ((q, k, k), dict(scale=float("inf")), "scale"),
+                           ((z(2, 10, 4, 16), k, k), {}, "q_start"), ((q, k, k), dict(q_start=-1), "q_start"), ((q, k, k), dict(lengths=[9, 9]), "lengths"),
+                           ((q, k, k), dict(lengths=n(9)), "lengths"), ((q, k, k), dict(lengths=n(9, 9, dtype=torch.int16)), "lengths"),
+                           ((q.double(), k.double(), k.double()), {}, "float32, float16 or bfloat16")):
+        with pytest.raises(GfppError, match=why):
+            window_attention(*args, **how)
+
+
+def test_step_refusals(no_launch):
+    q, k, c, p = z(2, 4, 16), z(2, 2, 16), z(2, 7, 2, 16), z(2, dtype=torch.int32)
+    ok = dict(q=q, k=k, v=k, cache_k=c, cache_v=c.clone(), positions=p, sinks=2)
+    with pytest.raises(Launched, match="gfpp_window_attn_step"):
+        window_attention_step(**ok)
+    for change, why in ((dict(cache_k=z(2, 7, 2, 8)), "cache_k"), (dict(cache_v=z(2, 6, 2, 16)), "cache_v"), (dict(cache_v=c.half()), "cache_v must be"),
+                        (dict(cache_k=z(2, 7, 16, 2).transpose(2, 3)), "dense last axis"), (dict(cache_k=z(1, 7, 2, 16).expand(2, 7, 2, 16)), "rows of its own"),
+                        (dict(sinks=7), "sinks"), (dict(sinks=-1), "sinks"), (dict(cache_k=c[:, :0], cache_v=c[:, :0], sinks=0), "sinks"), (dict(positions=p[:1]), "positions"),
+                        (dict(positions=p.float()), "positions"), (dict(positions=z(4, dtype=torch.int32)[::2]), "positions"), (dict(q=z(2, 4, 16).requires_grad_(True)), "no gradients"),
+                        (dict(scale=0), "scale"), (dict(q=z(2, 3, 16)), "multiple"), (dict(k=z(2, 2, 8), v=z(2, 2, 8)), "head width")):
+        with pytest.raises(GfppError, match=why):
+            window_attention_step(**{**ok, **change})
+    with pytest.raises(GfppError, match="window"):
+        WindowCache(1, 1, 8, 0, device="cpu")
+    cache = WindowCache(2, 1, 8, 4, 1, dtype=f32, device="cpu")
+    with pytest.raises(GfppError, match="k, v must be"):
+        cache.fill(z(2, 3, 1, 4), z(2, 3, 1, 4))
+    with pytest.raises(GfppError, match="torch.float32"):
+        cache.fill(z(2, 3, 1, 8, dtype=f16), z(2, 3, 1, 8, dtype=f16))
+    with pytest.raises(GfppError, match="lengths"):
+        cache.fill(z(2, 3, 1, 8), z(2, 3, 1, 8), torch.zeros(3, dtype=torch.int32))
+
+
+def test_fill_is_what_the_steps_leave():
+    """The ring arithmetic of WindowCache.fill on the CPU: the slot rule, token by token."""
+    g = torch.Generator().manual_seed(0)
+    for window, sinks in ((1, 0), (4, 0), (3, 2), (7, 1)):
+        for T in range(0, 20):
+            k, v = torch.randn(1, T, 1, 2, generator=g), torch.randn(1, T, 1, 2, generator=g)
+            cache = WindowCache(1, 1, 2, window, sinks, dtype=f32, device="cpu")
+            cache.fill(k, v)
+            want_k, want_v = torch.zeros_like(cache.k), torch.zeros_like(cache.v)
+            for n in range(T):
+                at = n if n < sinks else sinks + (n - sinks) % window
+                want_k[0, at], want_v[0, at] = k[0, n], v[0, n]
+            assert torch.equal(cache.k, want_k) and torch.equal(cache.v, want_v) and int(cache.positions) == T
+
+
+# ---- the C entry points: every bad call returns its code before a launch (the pointers are never followed) ------------------------------------------------------
+P, EINVAL, EUNSUPPORTED = 4096, -1, -2
+
+
+def test_c_entry_refusals():
+    lib = _lib.lib()
+    s = lambda n: (ctypes.c_int64 * n)(*[8] * n)  # noqa: E731
+    inf, nan = float("inf"), float("nan")
+
+    def norm(x=P, pitch=8, w=P, b=P, pt=0, M=4, N=8, eps=1e-5, dt=0, y=P, mean=None, rstd=None):
+        return lib.gfpp_layer_norm_forward(x, pitch, w, b, pt, M, N, eps, dt, y, mean, rstd, None)
+    for bad in (dict(dt=3), dict(dt=-1), dict(pt=1), dict(N=0), dict(N=2 ** 31), dict(mean=P), dict(rstd=P), dict(eps=-1.0), dict(eps=nan), dict(x=None), dict(y=None), dict(pitch=-8)):
+        assert norm(**bad) == EINVAL and b"gfpp_layer_norm_forward" in lib.gfpp_last_error(), bad
+    assert norm(M=0, x=None, y=None) == 0
+
+    def norm_bwd(dy=P, dyp=8, x=P, xp=8, w=P, pt=0, mean=P, rstd=P, M=4, N=8, dt=0, dx=P, dw=P, db=P, scratch=P):
+        return lib.gfpp_layer_norm_backward(dy, dyp, x, xp, w, pt, mean, rstd, M, N, dt, dx, dw, db, scratch, None)
+    for bad in (dict(dt=7), dict(pt=2), dict(N=0), dict(dy=None), dict(x=None), dict(mean=None), dict(rstd=None), dict(scratch=None), dict(xp=-1), dict(dyp=-1)):
+        assert norm_bwd(**bad) == EINVAL, bad
+    assert norm_bwd(dx=None, dw=None, db=None) == 0
+
+    def rotary(x0=P, h0=2, y0=P, x1=P, h1=1, y1=P, pos=P, pt=0, ps=0, f=P, sec=(2, 2), B=1, T=4, D=8, dt=0, s0=s(3), axes=None, s1=s(3)):
+        return lib.gfpp_rotary(x0, s0, h0, y0, x1, s1, h1, y1, pos, pt, ps, f, (ctypes.c_uint32 * max(1, len(sec)))(*sec), len(sec) if axes is None else axes, B, T, D, 0, 0, dt, None)
+    for bad in (dict(dt=3), dict(axes=0), dict(axes=5, sec=(1, 1, 1, 1, 1)), dict(sec=(2, 3)), dict(sec=(0, 0)), dict(sec=(2 ** 31, 2 ** 31)), dict(pt=3), dict(ps=-1), dict(x0=None),
+                dict(y0=None), dict(x1=None), dict(y1=None), dict(s0=None), dict(s1=None), dict(pos=None), dict(f=None), dict(D=2 ** 17), dict(h0=2 ** 17),
+                dict(h0=65536, h1=65536, D=1024), dict(B=2 ** 31, T=2 ** 31)):
+        assert rotary(**bad) == EINVAL, bad
+    assert rotary(T=0, pos=None) == 0 and rotary(h0=0, h1=0) == 0
+
+    def attn(q=P, k=P, v=P, o=P, st=s(12), B=1, Tq=4, Tk=4, Hq=2, Hk=1, D=8, left=3, right=0, sinks=0, start=0, scale=1.0, dt=0):
+        return lib.gfpp_window_attn_forward(q, k, v, o, None, st, B, Tq, Tk, Hq, Hk, D, left, right, sinks, start, None, scale, dt, None)
+    for bad in (dict(dt=3), dict(Hq=3, Hk=2), dict(Hk=0), dict(Hq=0), dict(left=-1), dict(right=-1), dict(sinks=-1), dict(start=-1), dict(start=2 ** 30), dict(Tq=2 ** 30),
+                dict(Tk=2 ** 30), dict(scale=0.0), dict(scale=-1.0), dict(scale=inf), dict(scale=nan), dict(q=None), dict(k=None), dict(v=None), dict(o=None), dict(st=None),
+                dict(B=2 ** 20, Tq=2 ** 20, Hq=64)):
+        assert attn(**bad) == EINVAL and b"gfpp_window_attn_forward" in lib.gfpp_last_error(), bad
+    assert attn(D=0) == attn(D=129) == EUNSUPPORTED and attn(B=0) == attn(Tq=0) == 0
+
+    def attn_bwd(q=P, k=P, v=P, o=P, g=P, lse=P, dq=P, dk=P, dv=P, scratch=P, st=s(24), B=1, Tq=4, Tk=4, Hq=2, Hk=1, D=8, left=3, right=0, sinks=0, start=0, scale=1.0, dt=0):
+        return lib.gfpp_window_attn_backward(q, k, v, o, g, lse, dq, dk, dv, scratch, st, B, Tq, Tk, Hq, Hk, D, left, right, sinks, start, None, scale, dt, None)
+    for name in ("q", "k", "v", "o", "g", "lse", "dq", "dk", "dv", "scratch", "st"):
+        assert attn_bwd(**{name: None}) == EINVAL, name
+    for bad in (dict(dt=9), dict(Hq=3, Hk=2), dict(left=-1), dict(scale=nan), dict(start=-5)):
+        assert attn_bwd(**bad) == EINVAL, bad
+    assert attn_bwd(D=200) == EUNSUPPORTED and attn_bwd(B=0) == 0
+    assert lib.gfpp_window_attn_backward_scratch_floats(2, 100, 100, 4, 2, 64, 10, 3, 0) == 2 * 4 * 100        # short: the sinks' tile is one workgroup's
+    assert lib.gfpp_window_attn_backward_scratch_floats(1, 4096, 4096, 4, 2, 64, 10, 3, 0) > 4 * 4096         # long: slices
+
+    def step(q=P, k=P, v=P, ck=P, cv=P, pos=P, o=P, st=s(14), B=1, Hq=2, Hk=1, D=8, slots=100, sinks=2, scale=1.0, dt=0, scratch=None):
+        return lib.gfpp_window_attn_step(q, k, v, ck, cv, pos, 0, o, st, B, Hq, Hk, D, slots, sinks, scale, dt, scratch, None)
+    for name in ("q", "k", "v", "ck", "cv", "pos", "o", "st"):
+        assert step(**{name: None}) == EINVAL, name
+    for bad in (dict(dt=3), dict(Hq=3, Hk=2), dict(Hk=0), dict(slots=0, sinks=0), dict(sinks=100), dict(scale=0.0), dict(slots=2 ** 30), dict(slots=100000, scratch=None)):
+        assert step(**bad) == EINVAL, bad
+    assert step(D=129) == EUNSUPPORTED and step(B=0) == 0
+    assert lib.gfpp_window_attn_step_scratch_floats(1, 2, 1, 8, 100000) > 0
