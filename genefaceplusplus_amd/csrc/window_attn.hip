@@ -15,7 +15,8 @@ namespace gfpp {
 template <typename T, int DP>
 constexpr int wa_bn() { return sizeof(T) == 4 && DP == 128 ? 32 : 64; }
 
-template <typename T, int DP, bool VEC>
+// TWO: probabilities as a rounded value and its remainder (window_attn_device.h: wa_two_part)
+template <typename T, int DP, bool VEC, bool TWO>
 __global__ __launch_bounds__(kWaThreads, sizeof(T) == 2 ? 2 : 1) void k_window_attn(WaArgs a) {
     constexpr int BN = wa_bn<T, DP>(), NS = DP / 16, NT = DP / 32, NSUB = BN / 32, PK = wa_pitch_row<T, DP>(), PV = wa_pitch_col<T, DP>();
     typedef typename LpTraits<T>::vec vec;
@@ -52,6 +53,7 @@ __global__ __launch_bounds__(kWaThreads, sizeof(T) == 2 ? 2 : 1) void k_window_a
             rv.load(vb, a.v.st, tile_row(1), n, a.D);
         }
     }
+    wa_arrived(q);
     __syncthreads();
     const int row_at = c * PK + 8 * h * (int)sizeof(T), col_at = wa_col_offset<T>(lane, PV);
     for (int k = 0; k < tiles; ++k) {
@@ -105,7 +107,7 @@ __global__ __launch_bounds__(kWaThreads, sizeof(T) == 2 ? 2 : 1) void k_window_a
             for (int u = 0; u < NSUB; ++u)
 #pragma unroll
                 for (int r = 0; r < 16; ++r) {
-                    s[u][r] = wa_prob<T>(s[u][r], top0, base, a.c);
+                    s[u][r] = wa_prob<TWO || sizeof(T) == 4>(s[u][r], top0, base, a.c);
                     l += s[u][r];
                 }
 #pragma unroll
@@ -115,6 +117,13 @@ __global__ __launch_bounds__(kWaThreads, sizeof(T) == 2 ? 2 : 1) void k_window_a
                     const vec pr = wa_pack<T>(s[u], x);
 #pragma unroll
                     for (int t = 0; t < NT; ++t) acc[t] = LpTraits<T>::mfma(wa_col<T, PV>(s_v[buf] + col_at, 32 * u + 16 * x, t), pr, acc[t]);
+                    if constexpr (TWO) {
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) s[u][8 * x + e] -= (float)pr[e];
+                        const vec rest = wa_pack<T>(s[u], x);
+#pragma unroll
+                        for (int t = 0; t < NT; ++t) acc[t] = LpTraits<T>::mfma(wa_col<T, PV>(s_v[buf] + col_at, 32 * u + 16 * x, t), rest, acc[t]);
+                    }
                 }
         }
         __syncthreads();
@@ -122,7 +131,10 @@ __global__ __launch_bounds__(kWaThreads, sizeof(T) == 2 ? 2 : 1) void k_window_a
     l = half_wave_sum(l);
     if (i >= a.Tq) return;
     T *o = static_cast<T *>(a.o.p) + b * a.o.sb + (int64_t)i * a.o.st + hq * a.o.sh;
-    wa_store_rows<T, NT, VEC>(acc, l > 0.0f ? 1.0f / l : 0.0f, o, h, a.D);
+    const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+    wa_store_rows<T, NT, VEC>(acc, inv, o, h, a.D);
+    if constexpr (TWO)
+        if (a.low) wa_store_rows<T, NT, VEC, true>(acc, inv, static_cast<T *>(a.low) + (o - static_cast<T *>(a.o.p)), h, a.D);
     // log2 of the row's sum, +inf for a row without visible keys: every probability of the backward pass is then exp2(-inf) = 0
     if (a.lse && h == 0) a.lse[((int64_t)b * a.Hq + hq) * a.Tq + i] = l > 0.0f ? m * a.c + log2f(l) : INFINITY;
 }
@@ -174,18 +186,20 @@ int wa_arguments(const char *what, WaArgs &a, const int64_t *strides, int n_tens
     return 0;
 }
 
-template <typename T>
+template <typename T, bool TWO>
 static void wa_forward(const WaArgs &a, bool vec, uint32_t grid, hipStream_t st) {
-    if (a.D <= 32) vec ? k_window_attn<T, 32, true><<<grid, kWaThreads, 0, st>>>(a) : k_window_attn<T, 32, false><<<grid, kWaThreads, 0, st>>>(a);
-    else if (a.D <= 64) vec ? k_window_attn<T, 64, true><<<grid, kWaThreads, 0, st>>>(a) : k_window_attn<T, 64, false><<<grid, kWaThreads, 0, st>>>(a);
-    else vec ? k_window_attn<T, 128, true><<<grid, kWaThreads, 0, st>>>(a) : k_window_attn<T, 128, false><<<grid, kWaThreads, 0, st>>>(a);
+    if (a.D <= 32) vec ? k_window_attn<T, 32, true, TWO><<<grid, kWaThreads, 0, st>>>(a) : k_window_attn<T, 32, false, TWO><<<grid, kWaThreads, 0, st>>>(a);
+    else if (a.D <= 64) vec ? k_window_attn<T, 64, true, TWO><<<grid, kWaThreads, 0, st>>>(a) : k_window_attn<T, 64, false, TWO><<<grid, kWaThreads, 0, st>>>(a);
+    else vec ? k_window_attn<T, 128, true, TWO><<<grid, kWaThreads, 0, st>>>(a) : k_window_attn<T, 128, false, TWO><<<grid, kWaThreads, 0, st>>>(a);
 }
 
 }  // namespace gfpp
 
 using namespace gfpp;
 
-GFPP_API int gfpp_window_attn_forward(const void *q, const void *k, const void *v, void *out, float *lse, const int64_t *strides, uint32_t B, uint32_t Tq, uint32_t Tk,
+GFPP_API int gfpp_window_attn_two_part(uint32_t Tk, int32_t left, int32_t right, int32_t sinks, int dtype) { return wa_two_part(Tk, left, right, sinks, dtype); }
+
+GFPP_API int gfpp_window_attn_forward(const void *q, const void *k, const void *v, void *out, void *out_low, float *lse, const int64_t *strides, uint32_t B, uint32_t Tq, uint32_t Tk,
                                       uint32_t Hq, uint32_t Hk, uint32_t D, int32_t left, int32_t right, int32_t sinks, int32_t q_start, const int32_t *lengths, float scale,
                                       int dtype, gfpp_stream_t stream) {
     const char *what = "gfpp_window_attn_forward";
@@ -198,13 +212,15 @@ GFPP_API int gfpp_window_attn_forward(const void *q, const void *k, const void *
     a.v.p = const_cast<void *>(v);
     a.o.p = out;
     a.lse = lse;
+    const bool two = wa_two_part(Tk, left, right, sinks, dtype);
+    a.low = two ? out_low : nullptr;
     const uint64_t grid = (uint64_t)div_up(Tq, kWaRows) * Hq * B;
     WA_REQUIRE(grid <= 0x7fffffffull);
     const size_t size = dtype == GFPP_F32 ? 4 : 2;
-    const bool vec = wa_vectors(a.q, a.D, size) && wa_vectors(a.k, a.D, size) && wa_vectors(a.v, a.D, size) && wa_vectors(a.o, a.D, size);
+    const bool vec = wa_vectors(a.q, a.D, size) && wa_vectors(a.k, a.D, size) && wa_vectors(a.v, a.D, size) && wa_vectors(a.o, a.D, size) && (uintptr_t)a.low % 16 == 0;
     hipStream_t st = (hipStream_t)stream;
-    if (dtype == GFPP_F32) wa_forward<float>(a, vec, (uint32_t)grid, st);
-    else if (dtype == GFPP_F16) wa_forward<_Float16>(a, vec, (uint32_t)grid, st);
-    else wa_forward<__bf16>(a, vec, (uint32_t)grid, st);
+    if (dtype == GFPP_F32) wa_forward<float, false>(a, vec, (uint32_t)grid, st);
+    else if (dtype == GFPP_F16) two ? wa_forward<_Float16, true>(a, vec, (uint32_t)grid, st) : wa_forward<_Float16, false>(a, vec, (uint32_t)grid, st);
+    else two ? wa_forward<__bf16, true>(a, vec, (uint32_t)grid, st) : wa_forward<__bf16, false>(a, vec, (uint32_t)grid, st);
     return check_launch(what);
 }

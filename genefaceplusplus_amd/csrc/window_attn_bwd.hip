@@ -41,6 +41,11 @@ __global__ __launch_bounds__(kWaThreads, sizeof(T) == 2 ? 2 : 1) void k_window_a
         wa_global_rows<T, NS, VEC>(o, static_cast<const T *>(a.o.p) + b * a.o.sb + (int64_t)i * a.o.st + hq * a.o.sh, have, h, a.D);
 #pragma unroll
         for (int x = 0; x < NS; ++x) d = LpTraits<T>::mfma(o[x], g[x], d);
+        if (a.low) {                                           // (wa_two_part: what the rounding of out took)
+            wa_global_rows<T, NS, VEC>(o, static_cast<const T *>(a.low) + b * a.o.sb + (int64_t)i * a.o.st + hq * a.o.sh, have, h, a.D);
+#pragma unroll
+            for (int x = 0; x < NS; ++x) d = LpTraits<T>::mfma(o[x], g[x], d);
+        }
         // the diagonal: column c's value of row c is in the half (c >> 2) & 1, register 4 (c >> 3) + (c & 3)
 #pragma unroll
         for (int r = 0; r < 16; ++r) delta = (4 * (c >> 3) + (c & 3)) == r ? d[r] : delta;
@@ -71,6 +76,8 @@ __global__ __launch_bounds__(kWaThreads, sizeof(T) == 2 ? 2 : 1) void k_window_a
             rv.load(vb, a.v.st, tile_row(1), n, a.D);
         }
     }
+    wa_arrived(q);
+    wa_arrived(g);
     __syncthreads();
     const int row_k = c * PK + 8 * h * (int)sizeof(T), row_v = c * PV + 8 * h * (int)sizeof(T), col_at = wa_col_offset<T>(lane, PK);
     for (int k = 0; k < tiles; ++k) {
@@ -86,31 +93,38 @@ __global__ __launch_bounds__(kWaThreads, sizeof(T) == 2 ? 2 : 1) void k_window_a
         const bool seen = pw0 < n && j0 <= pw1 + a.right && (j1 >= pw0 - a.left || j0 < a.sinks);
         if (seen) {
             const bool full = pw1 < n && j1 < n && j1 <= pw0 + a.right && (j0 >= pw1 - a.left || j1 < a.sinks);
+            // Two bodies without a branch inside: the products of one half tile may then overlap the arithmetic of the other.  The widest heads have no registers
+            // for two half tiles at once (two wavefronts per SIMD overlap instead): one body, the branch between its products.
+            auto body = [&](auto masked, auto always) {
 #pragma unroll
-            for (int u = 0; u < BN / 32; ++u) {
-                v16f s, d;
+                for (int u = 0; u < BN / 32; ++u) {
+                    v16f s, d;
 #pragma unroll
-                for (int r = 0; r < 16; ++r) s[r] = d[r] = 0.0f;
+                    for (int r = 0; r < 16; ++r) s[r] = d[r] = 0.0f;
 #pragma unroll
-                for (int x = 0; x < NS; ++x) s = LpTraits<T>::mfma(wa_row<T>(s_k[buf] + row_k + 32 * u * PK, x), q[x], s);
+                    for (int x = 0; x < NS; ++x) s = LpTraits<T>::mfma(wa_row<T>(s_k[buf] + row_k + 32 * u * PK, x), q[x], s);
 #pragma unroll
-                for (int x = 0; x < NS; ++x) d = LpTraits<T>::mfma(wa_row<T>(s_v[buf] + row_v + 32 * u * PV, x), g[x], d);
-                if (!full) {
+                    for (int x = 0; x < NS; ++x) d = LpTraits<T>::mfma(wa_row<T>(s_v[buf] + row_v + 32 * u * PV, x), g[x], d);
+                    if (decltype(masked)::value && (decltype(always)::value || !full)) {
 #pragma unroll
-                    for (int r = 0; r < 16; ++r) {
-                        const int j = j0 + 32 * u + 8 * (r >> 2) + 4 * h + (r & 3);
-                        s[r] = j <= last && (j >= first || j < a.sinks) ? s[r] : -INFINITY;
+                        for (int r = 0; r < 16; ++r) {
+                            const int j = j0 + 32 * u + 8 * (r >> 2) + 4 * h + (r & 3);
+                            s[r] = j <= last && (j >= first || j < a.sinks) ? s[r] : -INFINITY;
+                        }
+                    }
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], a.c, -lse)) * (d[r] - delta);
+#pragma unroll
+                    for (int x = 0; x < 2; ++x) {
+                        const vec ds = wa_pack<T>(s, x);
+#pragma unroll
+                        for (int t = 0; t < NT; ++t) acc[t] = LpTraits<T>::mfma(wa_col<T, PK>(s_k[buf] + col_at, 32 * u + 16 * x, t), ds, acc[t]);
                     }
                 }
-#pragma unroll
-                for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], a.c, -lse)) * (d[r] - delta);
-#pragma unroll
-                for (int x = 0; x < 2; ++x) {
-                    const vec ds = wa_pack<T>(s, x);
-#pragma unroll
-                    for (int t = 0; t < NT; ++t) acc[t] = LpTraits<T>::mfma(wa_col<T, PK>(s_k[buf] + col_at, 32 * u + 16 * x, t), ds, acc[t]);
-                }
-            }
+            };
+            if constexpr (DP == 128) body(WaFlag<true>{}, WaFlag<false>{});
+            else if (full) body(WaFlag<false>{}, WaFlag<false>{});
+            else body(WaFlag<true>{}, WaFlag<true>{});
         }
         __syncthreads();
     }
@@ -121,7 +135,7 @@ __global__ __launch_bounds__(kWaThreads, sizeof(T) == 2 ? 2 : 1) void k_window_a
 // sums), then the other tiles.
 template <typename T, int DP, bool VEC>
 __global__ __launch_bounds__(kWaThreads, 1) void k_window_attn_dkv(WaArgs a) {
-    constexpr int BQ = sizeof(T) == 2 && DP <= 64 ? 64 : 32, NS = DP / 16, NT = DP / 32, PITCH = wa_pitch_both<T, DP>();
+    constexpr int BQ = sizeof(T) == 2 ? 64 : 32, NS = DP / 16, NT = DP / 32, PITCH = wa_pitch_both<T, DP>();
     typedef typename LpTraits<T>::vec vec;
     typedef float f4 __attribute__((ext_vector_type(4)));
     __shared__ __attribute__((aligned(16))) unsigned char s_q[2][BQ * PITCH], s_g[2][BQ * PITCH];
@@ -185,6 +199,8 @@ __global__ __launch_bounds__(kWaThreads, 1) void k_window_attn_dkv(WaArgs a) {
         store(0);
         if (steps > 1) load(1);
     }
+    wa_arrived(kf);
+    wa_arrived(vf);
     __syncthreads();
     const int row_at = c * PITCH + 8 * h * (int)sizeof(T), col_at = wa_col_offset<T>(lane, PITCH);
     for (int k = 0; k < steps; ++k) {
@@ -196,42 +212,47 @@ __global__ __launch_bounds__(kWaThreads, 1) void k_window_attn_dkv(WaArgs a) {
         const bool seen = jw0 < n && p1 >= jw0 - a.right && (p0 <= jw1 + a.left || jw0 < a.sinks);
         if (seen) {
             const bool full = jw1 < n && p0 >= jw1 - a.right && (p1 <= jw0 + a.left || jw1 < a.sinks);
+            // (two bodies without a branch inside: the compiler overlaps the products of one sub-tile with the arithmetic of the other)
+            auto body = [&](auto masked) {
 #pragma unroll
-            for (int u = 0; u < BQ / 32; ++u) {
-                v16f s, d;
+                for (int u = 0; u < BQ / 32; ++u) {
+                    v16f s, d;
 #pragma unroll
-                for (int r = 0; r < 16; ++r) s[r] = d[r] = 0.0f;
+                    for (int r = 0; r < 16; ++r) s[r] = d[r] = 0.0f;
 #pragma unroll
-                for (int x = 0; x < NS; ++x) s = LpTraits<T>::mfma(wa_row<T>(s_q[buf] + row_at + 32 * u * PITCH, x), kf[x], s);
+                    for (int x = 0; x < NS; ++x) s = LpTraits<T>::mfma(wa_row<T>(s_q[buf] + row_at + 32 * u * PITCH, x), kf[x], s);
 #pragma unroll
-                for (int x = 0; x < NS; ++x) d = LpTraits<T>::mfma(wa_row<T>(s_g[buf] + row_at + 32 * u * PITCH, x), vf[x], d);
-                if (!full) {
-                    const int from = have ? j - a.right : 0x7fffffff, to = j < a.sinks ? 0x7fffffff : j + a.left;
+                    for (int x = 0; x < NS; ++x) d = LpTraits<T>::mfma(wa_row<T>(s_g[buf] + row_at + 32 * u * PITCH, x), vf[x], d);
+                    if constexpr (decltype(masked)::value) {
+                        const int from = have ? j - a.right : 0x7fffffff, to = j < a.sinks ? 0x7fffffff : j + a.left;
 #pragma unroll
-                    for (int r = 0; r < 16; ++r) {
-                        const int p = p0 + 32 * u + 8 * (r >> 2) + 4 * h + (r & 3);
-                        s[r] = p >= from && p <= to ? s[r] : -INFINITY;
+                        for (int r = 0; r < 16; ++r) {
+                            const int p = p0 + 32 * u + 8 * (r >> 2) + 4 * h + (r & 3);
+                            s[r] = p >= from && p <= to ? s[r] : -INFINITY;
+                        }
+                    }
+#pragma unroll
+                    for (int r = 0; r < 16; r += 4) {
+                        const f4 lse = *reinterpret_cast<const f4 *>(&s_lse[buf][32 * u + 2 * r + 4 * h]), delta = *reinterpret_cast<const f4 *>(&s_delta[buf][32 * u + 2 * r + 4 * h]);
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            s[r + e] = __builtin_amdgcn_exp2f(fmaf(s[r + e], a.c, -lse[e]));
+                            d[r + e] = s[r + e] * (d[r + e] - delta[e]);
+                        }
+                    }
+#pragma unroll
+                    for (int x = 0; x < 2; ++x) {
+                        const vec pr = wa_pack<T>(s, x), ds = wa_pack<T>(d, x);
+#pragma unroll
+                        for (int t = 0; t < NT; ++t) {
+                            dv[t] = LpTraits<T>::mfma(wa_col<T, PITCH>(s_g[buf] + col_at, 32 * u + 16 * x, t), pr, dv[t]);
+                            dk[t] = LpTraits<T>::mfma(wa_col<T, PITCH>(s_q[buf] + col_at, 32 * u + 16 * x, t), ds, dk[t]);
+                        }
                     }
                 }
-#pragma unroll
-                for (int r = 0; r < 16; r += 4) {
-                    const f4 lse = *reinterpret_cast<const f4 *>(&s_lse[buf][32 * u + 2 * r + 4 * h]), delta = *reinterpret_cast<const f4 *>(&s_delta[buf][32 * u + 2 * r + 4 * h]);
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        s[r + e] = __builtin_amdgcn_exp2f(fmaf(s[r + e], a.c, -lse[e]));
-                        d[r + e] = s[r + e] * (d[r + e] - delta[e]);
-                    }
-                }
-#pragma unroll
-                for (int x = 0; x < 2; ++x) {
-                    const vec pr = wa_pack<T>(s, x), ds = wa_pack<T>(d, x);
-#pragma unroll
-                    for (int t = 0; t < NT; ++t) {
-                        dv[t] = LpTraits<T>::mfma(wa_col<T, PITCH>(s_g[buf] + col_at, 32 * u + 16 * x, t), pr, dv[t]);
-                        dk[t] = LpTraits<T>::mfma(wa_col<T, PITCH>(s_q[buf] + col_at, 32 * u + 16 * x, t), ds, dk[t]);
-                    }
-                }
-            }
+            };
+            if (full) body(WaFlag<false>{});
+            else body(WaFlag<true>{});
         }
         __syncthreads();
     }
@@ -324,7 +345,7 @@ GFPP_API unsigned long long gfpp_window_attn_backward_scratch_floats(uint32_t B,
     return (unsigned long long)B * Hq * Tq + (unsigned long long)a.sink_tiles * a.splits * B * Hk * 2 * kWaRows * D;
 }
 
-GFPP_API int gfpp_window_attn_backward(const void *q, const void *k, const void *v, const void *out, const void *dout, const float *lse, void *dq, void *dk, void *dv,
+GFPP_API int gfpp_window_attn_backward(const void *q, const void *k, const void *v, const void *out, const void *out_low, const void *dout, const float *lse, void *dq, void *dk, void *dv,
                                        float *scratch, const int64_t *strides, uint32_t B, uint32_t Tq, uint32_t Tk, uint32_t Hq, uint32_t Hk, uint32_t D, int32_t left,
                                        int32_t right, int32_t sinks, int32_t q_start, const int32_t *lengths, float scale, int dtype, gfpp_stream_t stream) {
     const char *what = "gfpp_window_attn_backward";
@@ -341,6 +362,7 @@ GFPP_API int gfpp_window_attn_backward(const void *q, const void *k, const void 
     a.dq.p = dq;
     a.dk.p = dk;
     a.dv.p = dv;
+    a.low = wa_two_part(Tk, left, right, sinks, dtype) ? const_cast<void *>(out_low) : nullptr;
     a.lse = const_cast<float *>(lse);
     wa_bwd_setup(a);
     a.delta = scratch;
@@ -349,7 +371,7 @@ GFPP_API int gfpp_window_attn_backward(const void *q, const void *k, const void 
     const uint64_t gk = ((uint64_t)div_up(Tk, kWaRows) - a.sink_tiles + (uint64_t)a.sink_tiles * a.splits) * bh;
     WA_REQUIRE(gq <= 0x7fffffffull && gk <= 0x7fffffffull && (a.sink_tiles == 0 || (bh <= 65535 && a.sink_tiles <= 65535)));
     const size_t size = dtype == GFPP_F32 ? 4 : 2;
-    bool vec = true;
+    bool vec = (uintptr_t)a.low % 16 == 0;
     for (const WaTensor *t : {&a.q, &a.k, &a.v, &a.o, &a.dout, &a.dq, &a.dk, &a.dv}) vec = vec && wa_vectors(*t, a.D, size);
     hipStream_t st = (hipStream_t)stream;
     if (dtype == GFPP_F32) wa_backward<float>(a, vec, (uint32_t)gq, (uint32_t)gk, st);

@@ -16,12 +16,17 @@ namespace gfpp {
 
 constexpr int kWaThreads = 256, kWaRows = 128;      // four wavefronts of 32 queries (forward, dq) or 32 keys (dk, dv)
 
+template <bool B>
+struct WaFlag {
+    static constexpr bool value = B;
+};
 struct WaTensor {
     void *p;
     int64_t sb, st, sh;            // strides of sequence, token and head in elements
 };
 struct WaArgs {
     WaTensor q, k, v, o, dout, dq, dk, dv;
+    void *low;                     // out's rounding errors (o's strides), or NULL
     float *lse, *delta;            // [B][Hq][Tq]
     float *partial;                // sink tiles' dk and dv: [sink tiles][splits][B][Hk][2][128][D]
     const int32_t *lengths;        // [B] or NULL
@@ -161,6 +166,23 @@ __device__ __forceinline__ void wa_global_rows(typename LpTraits<T>::vec (&f)[NS
     }
 }
 
+// Has the fragments in their registers here.  Loads that are still in flight where a loop begins are otherwise waited for at their first use INSIDE it, in every
+// iteration, and with them the tile that the iteration has just requested.
+template <typename V, int N>
+__device__ __forceinline__ void wa_arrived(V (&f)[N]) {
+#pragma unroll
+    for (int x = 0; x < N; ++x) {
+        if constexpr (sizeof(V) == 16) {
+            asm volatile("" : "+v"(f[x]));
+        } else {
+            typedef float f4 __attribute__((ext_vector_type(4)));
+            f4 a = __builtin_shufflevector(f[x], f[x], 0, 1, 2, 3), b = __builtin_shufflevector(f[x], f[x], 4, 5, 6, 7);
+            asm volatile("" : "+v"(a), "+v"(b));
+            f[x] = __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+        }
+    }
+}
+
 // values 8 s .. 8 s + 7 of a product, rounded to the operand type (pairs: one conversion instruction each)
 template <typename T>
 __device__ __forceinline__ typename LpTraits<T>::vec wa_pack(const v16f &x, int s) {
@@ -182,11 +204,11 @@ __device__ __forceinline__ typename LpTraits<T>::vec wa_pack(const v16f &x, int 
     }
 }
 
-// exp2((s - m) c), base = m c.  16-bit modes: one fused multiply-add; its rounding of base is far below theirs.  fp32: the difference first, so that the largest
-// score's probability is exactly 1 and a query with one visible key copies its value
-template <typename T>
+// exp2((s - m) c), base = m c.  16-bit modes: one fused multiply-add; its rounding of base is far below theirs.  EXACT (fp32, two-part probabilities): the
+// difference first, so that the largest score's probability is exactly 1 and a query with one visible key copies its value
+template <bool EXACT>
 __device__ __forceinline__ float wa_prob(float s, float m, float base, float c) {
-    if constexpr (sizeof(T) == 4) return __builtin_amdgcn_exp2f((s - m) * c);
+    if constexpr (EXACT) return __builtin_amdgcn_exp2f((s - m) * c);
     return __builtin_amdgcn_exp2f(fmaf(s, c, -base));
 }
 
@@ -203,8 +225,16 @@ __device__ __forceinline__ T wa_scaled(float x, float f) {
     return (T)y;
 }
 
+// what rounding x f to T leaves of it
+template <typename T>
+__device__ __forceinline__ T wa_remainder(float x, float f) {
+    float y = x * f;
+    asm("" : "+v"(y));
+    return (T)(y - (float)(T)y);
+}
+
 // a product tile [32 T rows = features][32 columns = tokens] to the lane's token row: 4 consecutive features per store
-template <typename T, int NT, bool VEC>
+template <typename T, int NT, bool VEC, bool LOW = false>
 __device__ __forceinline__ void wa_store_rows(const v16f (&acc)[NT], float f, T *row, int h, int D) {
     typedef T vec4 __attribute__((ext_vector_type(4)));
 #pragma unroll
@@ -216,7 +246,7 @@ __device__ __forceinline__ void wa_store_rows(const v16f (&acc)[NT], float f, T 
             if (VEC || col + 3 < D) {
                 vec4 v;
 #pragma unroll
-                for (int e = 0; e < 4; ++e) v[e] = wa_scaled<T>(acc[t][r + e], f);
+                for (int e = 0; e < 4; ++e) v[e] = LOW ? wa_remainder<T>(acc[t][r + e], f) : wa_scaled<T>(acc[t][r + e], f);
                 if constexpr (VEC) {
                     *reinterpret_cast<vec4 *>(row + col) = v;
                 } else {
@@ -226,9 +256,18 @@ __device__ __forceinline__ void wa_store_rows(const v16f (&acc)[NT], float f, T 
             } else {
 #pragma unroll
                 for (int e = 0; e < 4; ++e)
-                    if (col + e < D) row[col + e] = wa_scaled<T>(acc[t][r + e], f);
+                    if (col + e < D) row[col + e] = LOW ? wa_remainder<T>(acc[t][r + e], f) : wa_scaled<T>(acc[t][r + e], f);
             }
         }
+}
+
+// The two-part rule.  Rounding a probability costs half a step of its weight; over many keys these errors average out below the output's own rounding, over few they
+// do not, and delta, the backward pass' row sum, carries both into every score gradient of the row.  Where a query sees at most 64 keys the forward pass therefore
+// takes its probabilities as a rounded value and a rounded remainder (a second product: such calls are bound by latency and memory), and a training pass keeps
+// the output's remainder for delta.  Goes by the arguments alone, so that a pass with gradients and one without give the same bits.
+__host__ __device__ inline bool wa_two_part(int64_t Tk, int64_t left, int64_t right, int64_t sinks, int dtype) {
+    const int64_t window = left + right + 1 + sinks;
+    return dtype != GFPP_F32 && (window < Tk ? window : Tk) <= 64;
 }
 
 // tiles of BN keys that queries at positions p0 .. p1 can see: [0, head) for the sinks in front of the band, [lo, hi) for the band (merged where they touch)

@@ -88,6 +88,7 @@ __global__ __launch_bounds__(kWaThreads, sizeof(T) == 2 ? 2 : 1) void k_window_a
     unsigned char *mine = lds + wave * 32 * PV;
     const int col_at = wa_col_offset<T>(lane, PV);
     int row0 = s0 + wave * 32;
+    wa_arrived(q);
     if (row0 < s1) load(row0);
     for (; row0 < s1; row0 += 128) {
         // (the wavefront's own tile: the LDS serves a wavefront's accesses in the order of its instructions, no barrier -- the fences hold the compiler to it)
@@ -124,7 +125,7 @@ __global__ __launch_bounds__(kWaThreads, sizeof(T) == 2 ? 2 : 1) void k_window_a
         const float top0 = m == -INFINITY ? 0.0f : m, base = top0 * a.c;
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
-            s[r] = wa_prob<T>(s[r], top0, base, a.c);
+            s[r] = wa_prob<sizeof(T) == 4>(s[r], top0, base, a.c);
             l += s[r];
         }
 #pragma unroll

@@ -9,16 +9,12 @@ total-variation gradient); SH and frequency encodings are forward only (their in
 Rotary positions (rotary_embed / RotaryEncoder, no counterpart in the reference) are the encoding of the sequence operators (sequence.py): they turn the heads of
 queries and keys by the tokens' positions on one or several axes.
 """
-import ctypes
-
 import numpy as np
 import torch
 import torch.nn as nn
-from torch.autograd.function import once_differentiable
 
-from .. import _lib
+from . import sequence
 from .._lib import call, GfppError
-from .sequence import DTYPES, check_tensors, launch, wants_grad
 
 _GRIDTYPE = {"hash": 0, "tiled": 1}
 _INTERP = {"linear": 0, "smoothstep": 1}
@@ -283,72 +279,15 @@ class FreqEncoder(nn.Module):
         return out.view(prefix + [self.output_dim])
 
 
-_lib.register("gfpp_rotary", [ctypes.c_void_p, ctypes.POINTER(ctypes.c_int64), ctypes.c_uint32, ctypes.c_void_p] * 2
-              + [ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c_void_p, ctypes.POINTER(ctypes.c_uint32)] + [ctypes.c_uint32] * 4
-              + [ctypes.c_int] * 3 + [ctypes.c_void_p])
-_POSITIONS = {torch.int32: 0, torch.int64: 1, torch.float32: 2}
-
-
-def _rotary_launch(tensors, positions, frequencies, sections, interleaved, backward):
-    B, T, _, D = tensors[0].shape
-    out, args = [], []
-    for t in tensors:
-        t = t if t.stride(3) == 1 else t.contiguous()
-        y = torch.empty(t.shape, dtype=t.dtype, device=t.device)
-        args += [t.data_ptr(), (ctypes.c_int64 * 3)(*t.stride()[:3]), t.shape[2], y.data_ptr()]
-        out.append(y)
-    if len(tensors) == 1:
-        args += [None, None, 0, None]
-    launch(tensors[0].device, "gfpp_rotary", *args, positions.data_ptr(), _POSITIONS[positions.dtype], positions.stride(0) if positions.dim() == 3 else 0,
-           frequencies.data_ptr(), (ctypes.c_uint32 * len(sections))(*sections), len(sections), B, T, D, int(interleaved), int(backward), DTYPES[tensors[0].dtype])
-    return tuple(out)
-
-
-class _RotaryFn(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, positions, frequencies, sections, interleaved, *tensors):
-        ctx.save_for_backward(positions, frequencies)
-        ctx.how = (sections, interleaved)
-        return _rotary_launch(tensors, positions, frequencies, sections, interleaved, False)
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, *grads):
-        # the transpose of a turn is the turn by the opposite angle (a tensor that needs no gradient still takes its place in the launch: they come in pairs)
-        positions, frequencies = ctx.saved_tensors
-        return (None, None, None, None) + _rotary_launch(grads, positions, frequencies, *ctx.how, True)
-
-
 def rotary_embed(x, positions, frequencies, sections, interleaved=False):
     """Turns pairs of features by the tokens' positions: x [B, T, H, D], or a pair of such tensors (queries and keys, other H) that go through in one launch.
 
     sections: pairs of every axis, 1 .. 4 axes; the first 2 P features of a head, P = sum(sections), are P pairs -- (i, i + P), or (2 i, 2 i + 1) when
     interleaved -- and pair i of axis a is turned by ``positions[..., a] * frequencies[i]`` radians; the features behind pass through.  positions: [T, axes] or
     [B, T, axes], int32, int64 or float32; frequencies: [P] float64 (angles are taken in 64 bits: exact at far positions).  Differentiable in x."""
-    pair = isinstance(x, (tuple, list))
-    tensors = tuple(x) if pair else (x,)
-    if not 1 <= len(tensors) <= 2:
-        raise GfppError(f"rotary_embed: one tensor or two, got {len(tensors)}")
-    first = tensors[0]
-    check_tensors("rotary_embed", first, positions=positions, frequencies=frequencies, **({"keys": tensors[1]} if len(tensors) == 2 else {}))
-    sections = tuple(int(n) for n in sections)
-    P = sum(sections)
-    for t in tensors:
-        if t.dim() != 4 or t.dtype != first.dtype or (t.shape[0], t.shape[1], t.shape[3]) != (first.shape[0], first.shape[1], first.shape[3]):
-            raise GfppError(f"rotary_embed: [B, T, H, D] tensors of one type that differ in H alone, got {[tuple(u.shape) for u in tensors]}")
-    B, T, _, D = first.shape
-    if not 1 <= len(sections) <= 4 or min(sections) < 0 or not 1 <= P <= 512 or 2 * P > D:
-        raise GfppError(f"rotary_embed: sections {sections}: 1 .. 4 axes, 1 .. 512 pairs, {D} features")
-    if positions.dtype not in _POSITIONS or tuple(positions.shape) not in ((T, len(sections)), (B, T, len(sections))):
-        raise GfppError(f"rotary_embed: positions must be int32, int64 or float32 [{T}, {len(sections)}] or [{B}, {T}, {len(sections)}], got {positions.dtype} {tuple(positions.shape)}")
-    if frequencies.dtype != torch.float64 or tuple(frequencies.shape) != (P,):
-        raise GfppError(f"rotary_embed: frequencies must be float64 [{P}], got {frequencies.dtype} {tuple(frequencies.shape)}")
-    positions, frequencies = positions.contiguous(), frequencies.contiguous()
-    if wants_grad(*tensors):
-        out = _RotaryFn.apply(positions, frequencies, sections, bool(interleaved), *tensors)
-    else:
-        out = _rotary_launch(tensors, positions, frequencies, sections, interleaved, False)
-    return out if pair else out[0]
+    if isinstance(x, torch.Tensor):
+        return (sequence._ops or sequence.ops()).rotary_embed((x,), positions, frequencies, sections, interleaved)[0]
+    return tuple((sequence._ops or sequence.ops()).rotary_embed(x, positions, frequencies, sections, interleaved))
 
 
 class RotaryEncoder(nn.Module):

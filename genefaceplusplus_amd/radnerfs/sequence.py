@@ -5,12 +5,13 @@ a conditioning network over whole clips (thousands of frames, forward and backwa
 them are in encoders.py.  Hand-written HIP kernels through the C ABI (csrc/layer_norm.hip, window_attn*.hip); float32, float16 and bfloat16, sums in float32.
 
 Tensors live on one GPU, nothing is moved silently; kernels run on torch's current stream of that GPU.  Gradients are first derivatives only, summed in a fixed
-order (the same bits every time)."""
+order (the same bits every time).  Argument checks, allocation and the autograd nodes are compiled (csrc/sequence_torch.cpp)."""
 import ctypes
+import importlib
+import os
 
 import torch
 import torch.nn as nn
-from torch.autograd.function import once_differentiable
 
 from .. import _lib
 from .._lib import GfppError
@@ -20,121 +21,39 @@ _strides = ctypes.POINTER(ctypes.c_int64)
 _lib.register("gfpp_layer_norm_forward", [_p, _i64, _p, _p, _i, _u64, _u32, _f, _i, _p, _p, _p, _p])
 _lib.register("gfpp_layer_norm_backward", [_p, _i64, _p, _i64, _p, _i, _p, _p, _u64, _u32, _i, _p, _p, _p, _p, _p])
 _lib.register("gfpp_layer_norm_backward_scratch_floats", [_u64, _u32], restype=ctypes.c_uint64)
-_lib.register("gfpp_window_attn_forward", [_p, _p, _p, _p, _p, _strides] + [_u32] * 6 + [_i32] * 4 + [_p, _f, _i, _p])
-_lib.register("gfpp_window_attn_backward", [_p] * 10 + [_strides] + [_u32] * 6 + [_i32] * 4 + [_p, _f, _i, _p])
+_lib.register("gfpp_rotary", [_p, _strides, _u32, _p] * 2 + [_p, _i, _i64, _p, ctypes.POINTER(_u32)] + [_u32] * 4 + [_i] * 3 + [_p])
+_lib.register("gfpp_window_attn_two_part", [_u32] + [_i32] * 3 + [_i])
+_lib.register("gfpp_window_attn_forward", [_p] * 6 + [_strides] + [_u32] * 6 + [_i32] * 4 + [_p, _f, _i, _p])
+_lib.register("gfpp_window_attn_backward", [_p] * 11 + [_strides] + [_u32] * 6 + [_i32] * 4 + [_p, _f, _i, _p])
 _lib.register("gfpp_window_attn_backward_scratch_floats", [_u32] * 6 + [_i32] * 3, restype=ctypes.c_uint64)
 _lib.register("gfpp_window_attn_step", [_p] * 6 + [_i, _p, _strides] + [_u32] * 6 + [_f, _i, _p, _p])
 _lib.register("gfpp_window_attn_step_scratch_floats", [_u32] * 5, restype=ctypes.c_uint64)
-
-DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
-#: a window side without an end
-_FAR = 1 << 29
-
-
-def launch(device, name, *args):
-    """One entry point on `device` and torch's current stream there, whatever the current device is."""
-    if device.index == torch.cuda.current_device():
-        _lib.call(name, *args, torch.cuda.current_stream().cuda_stream)
-    else:
-        with torch.cuda.device(device):
-            _lib.call(name, *args, torch.cuda.current_stream().cuda_stream)
+_SYMBOLS = ("gfpp_last_error", "gfpp_layer_norm_forward", "gfpp_layer_norm_backward", "gfpp_layer_norm_backward_scratch_floats", "gfpp_rotary", "gfpp_window_attn_two_part",
+            "gfpp_window_attn_forward", "gfpp_window_attn_backward", "gfpp_window_attn_backward_scratch_floats", "gfpp_window_attn_step",
+            "gfpp_window_attn_step_scratch_floats")
+_ops = None
 
 
-def scratch_floats(device, name, *args):
-    """The library's answer goes by the device's compute units."""
-    if device.index == torch.cuda.current_device():
-        return int(getattr(_lib.lib(), name)(*args))
-    with torch.cuda.device(device):
-        return int(getattr(_lib.lib(), name)(*args))
-
-
-def check_tensors(what, like, **tensors):
-    """Every given tensor on the GPU of `like` (the first one), of a supported type."""
-    if not like.is_cuda:
-        raise GfppError(f"{what}: tensors must be on the GPU (no CPU path)")
-    if like.dtype not in DTYPES:
-        raise GfppError(f"{what}: float32, float16 or bfloat16 expected, got {like.dtype}")
-    for name, t in tensors.items():
-        if t is not None and t.device != like.device:
-            raise GfppError(f"{what}: {name} is on {t.device}, expected {like.device}")
-
-
-def wants_grad(*tensors):
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
-
-
-def _ptr(t):
-    return None if t is None else t.data_ptr()
+def ops():
+    """The compiled binding (csrc/sequence_torch.cpp), given the entry points of the library that _lib has loaded.  Raises if it has not been built."""
+    global _ops
+    if _ops is None:
+        library = _lib.lib()
+        path = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "_sequence.so")
+        if not os.path.exists(path):
+            raise GfppError(f"{path} is missing: run `python -c 'import __graft_entry__ as g; g.build()'` (or `make -C genefaceplusplus_amd/csrc`). There is no fallback.")
+        module = importlib.import_module("genefaceplusplus_amd._sequence")
+        module.bind({name: ctypes.cast(getattr(library, name), ctypes.c_void_p).value for name in _SYMBOLS})
+        _ops = module
+    return _ops
 
 
 # ---- layer norm ------------------------------------------------------------------------------------------------------------------------------------------
-def _rows(t, N):
-    """t as [M, N] rows of one pitch: a view where the layout has one, a copy otherwise."""
-    if t.dim() == 2 and t.stride(1) == 1 and t.stride(0) >= 0:
-        return t
-    return t.contiguous().view(-1, N)
-
-
-def _layer_norm_forward(x, weight, bias, eps, keep):
-    N = x.shape[-1]
-    rows = _rows(x, N)
-    M = rows.shape[0]
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    stats = torch.empty(2, M, dtype=torch.float32, device=x.device) if keep else None
-    param = weight if weight is not None else bias
-    launch(x.device, "gfpp_layer_norm_forward", rows.data_ptr(), rows.stride(0), _ptr(weight), _ptr(bias), DTYPES[param.dtype] if param is not None else 0, M, N,
-           float(eps), DTYPES[x.dtype], y.data_ptr(), stats.data_ptr() if keep else None, stats[1].data_ptr() if keep else None)
-    return y, rows, stats
-
-
-class _LayerNormFn(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, weight, bias, eps):
-        y, rows, stats = _layer_norm_forward(x, weight, bias, eps, True)
-        ctx.save_for_backward(rows, weight, bias, stats)
-        return y
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dy):
-        rows, weight, bias, stats = ctx.saved_tensors
-        M, N = rows.shape
-        dev = rows.device
-        dyr = _rows(dy, N)
-        param = weight if weight is not None else bias
-        want_x, want_w, want_b = ctx.needs_input_grad[:3]
-        dx = torch.empty(dy.shape, dtype=rows.dtype, device=dev) if want_x else None
-        dw, db = torch.empty_like(weight) if want_w else None, torch.empty_like(bias) if want_b else None
-        scratch = None
-        if want_w or want_b:
-            scratch = torch.empty(scratch_floats(dev, "gfpp_layer_norm_backward_scratch_floats", M, N), dtype=torch.float32, device=dev)
-        launch(dev, "gfpp_layer_norm_backward", dyr.data_ptr(), dyr.stride(0), rows.data_ptr(), rows.stride(0), _ptr(weight),
-               DTYPES[param.dtype] if param is not None else 0, stats.data_ptr(), stats[1].data_ptr(), M, N, DTYPES[rows.dtype], _ptr(dx), _ptr(dw), _ptr(db),
-               _ptr(scratch))
-        return dx, dw, db, None
-
-
 def layer_norm(x, weight=None, bias=None, eps=1e-5):
     """(x - mean) / sqrt(var + eps) * weight + bias over the last axis of x [..., N]; differentiable in x, weight and bias.
 
     weight, bias: [N], float32 or x's type (both the same), or None.  The output has x's type; statistics and sums are float32."""
-    check_tensors("layer_norm", x, weight=weight, bias=bias)
-    if x.dim() < 1 or x.shape[-1] < 1:
-        raise GfppError(f"layer_norm: the last axis must not be empty, got {tuple(x.shape)}")
-    for name, p in (("weight", weight), ("bias", bias)):
-        if p is None:
-            continue
-        if tuple(p.shape) != (x.shape[-1],) or not p.is_contiguous():
-            raise GfppError(f"layer_norm: {name} must be a contiguous [{x.shape[-1]}], got {tuple(p.shape)}")
-        if p.dtype not in (torch.float32, x.dtype):
-            raise GfppError(f"layer_norm: {name} must be float32 or {x.dtype}, got {p.dtype}")
-    if weight is not None and bias is not None and weight.dtype != bias.dtype:
-        raise GfppError(f"layer_norm: weight is {weight.dtype}, bias {bias.dtype}")
-    if not eps >= 0:
-        raise GfppError(f"layer_norm: eps must not be negative, got {eps}")
-    if wants_grad(x, weight, bias):
-        return _LayerNormFn.apply(x, weight, bias, eps)
-    return _layer_norm_forward(x, weight, bias, eps, False)[0]
+    return (_ops or ops()).layer_norm(x, weight, bias, eps)
 
 
 class LayerNorm(nn.Module):
@@ -151,74 +70,6 @@ class LayerNorm(nn.Module):
 
 
 # ---- attention with a sliding window and sinks ---------------------------------------------------------------------------------------------------------------
-def _heads(t):
-    """t [B, T, H, D] with a dense last axis."""
-    return t if t.stride(3) == 1 or t.shape[3] == 1 else t.contiguous()
-
-
-def _token_strides(*tensors):
-    flat = [s for t in tensors for s in t.stride()[:3]]
-    return (ctypes.c_int64 * len(flat))(*flat)
-
-
-def _window_forward(q, k, v, window, lengths, scale, keep):
-    B, Tq, Hq, D = q.shape
-    Tk, Hk = k.shape[1], k.shape[2]
-    out = torch.empty(B, Tq, Hq, D, dtype=q.dtype, device=q.device)
-    lse = torch.empty(B, Hq, Tq, dtype=torch.float32, device=q.device) if keep else None
-    launch(q.device, "gfpp_window_attn_forward", q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), _ptr(lse), _token_strides(q, k, v, out), B, Tq, Tk, Hq, Hk,
-           D, *window, _ptr(lengths), scale, DTYPES[q.dtype])
-    return out, lse
-
-
-class _WindowAttentionFn(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, q, k, v, window, lengths, scale):
-        out, lse = _window_forward(q, k, v, window, lengths, scale, True)
-        ctx.save_for_backward(q, k, v, out, lse, lengths)
-        ctx.window, ctx.scale = window, scale
-        return out
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dout):
-        q, k, v, out, lse, lengths = ctx.saved_tensors
-        B, Tq, Hq, D = q.shape
-        Tk, Hk = k.shape[1], k.shape[2]
-        dev = q.device
-        dout = _heads(dout)
-        dq = torch.empty(q.shape, dtype=q.dtype, device=dev)
-        dk, dv = torch.empty(k.shape, dtype=k.dtype, device=dev), torch.empty(v.shape, dtype=v.dtype, device=dev)
-        left, right, sinks, start = ctx.window
-        scratch = torch.empty(scratch_floats(dev, "gfpp_window_attn_backward_scratch_floats", B, Tq, Tk, Hq, Hk, D, left, sinks, start), dtype=torch.float32, device=dev)
-        launch(dev, "gfpp_window_attn_backward", q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), dout.data_ptr(), lse.data_ptr(), dq.data_ptr(),
-               dk.data_ptr(), dv.data_ptr(), scratch.data_ptr(), _token_strides(q, k, v, out, dout, dq, dk, dv), B, Tq, Tk, Hq, Hk, D, *ctx.window, _ptr(lengths),
-               ctx.scale, DTYPES[q.dtype])
-        return dq, dk, dv, None, None, None
-
-
-def _check_heads(what, q, k, v, axes):
-    check_tensors(what, q, k=k, v=v)
-    if q.dim() != axes or k.dim() != axes or tuple(k.shape) != tuple(v.shape):
-        raise GfppError(f"{what}: q, k, v must have {axes} axes and k the shape of v, got {tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)}")
-    if k.dtype != q.dtype or v.dtype != q.dtype:
-        raise GfppError(f"{what}: q, k, v must have one type, got {q.dtype}, {k.dtype}, {v.dtype}")
-    if q.shape[0] != k.shape[0] or q.shape[-1] != k.shape[-1]:
-        raise GfppError(f"{what}: q and k differ in batch or head width: {tuple(q.shape)}, {tuple(k.shape)}")
-    Hq, Hk, D = q.shape[-2], k.shape[-2], q.shape[-1]
-    if Hk < 1 or Hq < 1 or Hq % Hk:
-        raise GfppError(f"{what}: {Hq} query heads are no multiple of {Hk} key heads")
-    if not 1 <= D <= 128:
-        raise GfppError(f"{what}: head width {D} (1 .. 128 are supported)")
-
-
-def _scale(what, scale, D):
-    scale = float(D) ** -0.5 if scale is None else float(scale)
-    if not 0.0 < scale < float("inf"):
-        raise GfppError(f"{what}: scale must be positive, got {scale}")
-    return scale
-
-
 def window_attention(q, k, v, left=None, right=0, sinks=0, lengths=None, scale=None, q_start=None):
     """softmax(scale q k^T) v over the keys that each query sees; differentiable in q, k and v.
 
@@ -227,28 +78,7 @@ def window_attention(q, k, v, left=None, right=0, sinks=0, lengths=None, scale=N
     q_start: Tk - Tq by default (the queries are the last tokens).  lengths: [B] int32 / int64 on the GPU, tokens of every sequence: what lies behind is neither
     read nor seen, its output rows and gradients are zero, as are those of a query that sees nothing.  Within its length a sequence has to be finite.
     scale: D ** -0.5 by default."""
-    what = "window_attention"
-    _check_heads(what, q, k, v, 4)
-    B, Tq, Tk = q.shape[0], q.shape[1], k.shape[1]
-    for name, n in (("left", left), ("right", right), ("sinks", sinks)):
-        if n is not None and (n != int(n) or n < 0):
-            raise GfppError(f"{what}: {name} must be a whole number from 0, got {n}")
-    if max(Tq, Tk, B) > _FAR:
-        raise GfppError(f"{what}: more than 2^29 tokens or sequences")
-    q_start = Tk - Tq if q_start is None else int(q_start)
-    if not 0 <= q_start <= _FAR:
-        raise GfppError(f"{what}: q_start {q_start} must be 0 .. 2^29 (more queries than keys need it given)")
-    if lengths is not None:
-        if not torch.is_tensor(lengths) or tuple(lengths.shape) != (B,) or lengths.dtype not in (torch.int32, torch.int64):
-            raise GfppError(f"{what}: lengths must be an int32 or int64 tensor [{B}]")
-        check_tensors(what, q, lengths=lengths)
-        lengths = lengths.clamp(0, Tk).to(torch.int32) if lengths.dtype == torch.int64 else lengths.contiguous()
-    window = (_FAR if left is None else min(int(left), _FAR), _FAR if right is None else min(int(right), _FAR), min(int(sinks or 0), _FAR), q_start)
-    scale = _scale(what, scale, q.shape[3])
-    q, k, v = _heads(q), _heads(k), _heads(v)
-    if wants_grad(q, k, v):
-        return _WindowAttentionFn.apply(q, k, v, window, lengths, scale)
-    return _window_forward(q, k, v, window, lengths, scale, False)[0]
+    return (_ops or ops()).window_attention(q, k, v, left, right, sinks, lengths, scale, q_start)
 
 
 def window_attention_step(q, k, v, cache_k, cache_v, positions, sinks=0, scale=None):
@@ -258,36 +88,7 @@ def window_attention_step(q, k, v, cache_k, cache_v, positions, sinks=0, scale=N
     and its last W = slots - sinks ones, the token at position n in slot ``n if n < sinks else sinks + (n - sinks) % W``.  positions: [B] int32 / int64 on the GPU, the
     new tokens' positions; a negative one leaves its stream as it is (output zeros).  The result is row n of window_attention(left=W - 1, right=0, sinks=sinks)
     over the whole stream.  Serving only: no gradients.  Positions and caches are read on the GPU, so a captured graph of steps can be replayed."""
-    what = "window_attention_step"
-    _check_heads(what, q, k, v, 3)
-    B, Hq, D = q.shape
-    Hk = k.shape[1]
-    check_tensors(what, q, cache_k=cache_k, cache_v=cache_v, positions=positions)
-    for name, c in (("cache_k", cache_k), ("cache_v", cache_v)):
-        if c.dim() != 4 or (c.shape[0], c.shape[2], c.shape[3]) != (B, Hk, D) or tuple(c.shape) != tuple(cache_k.shape):
-            raise GfppError(f"{what}: {name} must be [{B}, slots, {Hk}, {D}] like the other, got {tuple(c.shape)}")
-        if c.dtype != q.dtype:
-            raise GfppError(f"{what}: {name} must be {q.dtype}, got {c.dtype}")
-        if (D > 1 and c.stride(3) != 1) or any(s <= 0 and n > 1 for s, n in zip(c.stride(), c.shape)):
-            raise GfppError(f"{what}: {name} needs a dense last axis and rows of its own (strides {c.stride()}): it is written in place")
-    slots = cache_k.shape[1]
-    if sinks != int(sinks) or not 0 <= sinks < slots:
-        raise GfppError(f"{what}: sinks {sinks} must be 0 .. slots - 1 ({slots} slots)")
-    if slots > _FAR:
-        raise GfppError(f"{what}: more than 2^29 slots")
-    if tuple(positions.shape) != (B,) or positions.dtype not in (torch.int32, torch.int64) or not positions.is_contiguous():
-        raise GfppError(f"{what}: positions must be a contiguous int32 or int64 tensor [{B}]")
-    if wants_grad(q, k, v, cache_k, cache_v):
-        raise GfppError(f"{what}: no gradients (call it under torch.no_grad(); window_attention is the differentiable form)")
-    scale = _scale(what, scale, D)
-    q, k, v = (t if t.stride(2) == 1 or D == 1 else t.contiguous() for t in (q, k, v))
-    out = torch.empty(B, Hq, D, dtype=q.dtype, device=q.device)
-    n = scratch_floats(q.device, "gfpp_window_attn_step_scratch_floats", B, Hq, Hk, D, slots)
-    scratch = torch.empty(n, dtype=torch.float32, device=q.device) if n else None
-    strides = (ctypes.c_int64 * 14)(*q.stride()[:2], *k.stride()[:2], *v.stride()[:2], *cache_k.stride()[:3], *cache_v.stride()[:3], *out.stride()[:2])
-    launch(q.device, "gfpp_window_attn_step", q.data_ptr(), k.data_ptr(), v.data_ptr(), cache_k.data_ptr(), cache_v.data_ptr(), positions.data_ptr(),
-           int(positions.dtype == torch.int64), out.data_ptr(), strides, B, Hq, Hk, D, slots, int(sinks), scale, DTYPES[q.dtype], _ptr(scratch))
-    return out
+    return (_ops or ops()).window_attention_step(q, k, v, cache_k, cache_v, positions, sinks, scale)
 
 
 class WindowCache:

@@ -873,14 +873,17 @@ int gfpp_rotary(const void *x0, const int64_t *x0_strides, uint32_t heads0, void
 /* Attention with a sliding window and visible first tokens over a conditioning sequence (AudioAttNet's weighted window, cond_encoder.py:146-180, for sequences of any
  * length): out[b, i, h] = sum_j softmax_j(scale q[b, i, h] . k[b, j, h / G]) v[b, j, h / G], G = Hq / Hk, over the keys j that the query at position p = q_start + i
  * sees:  j < n and p < n and j <= p + right and (j >= p - left or j < sinks),  n = min(lengths[b], Tk) (lengths NULL: Tk).  A query that sees nothing gives
- * zeros.  q, out [B, Tq, Hq, D]; k, v [B, Tk, Hk, D]; strides: {B, T, H} of q, k, v, out; D 1 .. 128.  lse [B, Hq, Tq] f32 for the backward pass, or NULL.
+ * zeros.  out_low: NULL, or where gfpp_window_attn_two_part says so (16-bit types, few visible keys) a tensor with out's strides that takes what out's rounding left,
+ * for the backward pass.  q, out [B, Tq, Hq, D]; k, v [B, Tk, Hk, D]; strides: {B, T, H} of q, k, v, out; D 1 .. 128.  lse [B, Hq, Tq] f32 for the backward pass, or NULL.
  * Rows behind a sequence's length are not read (they may hold anything); within it keys and values have to be finite. */
-int gfpp_window_attn_forward(const void *q, const void *k, const void *v, void *out, float *lse, const int64_t *strides, uint32_t B, uint32_t Tq, uint32_t Tk,
+int gfpp_window_attn_forward(const void *q, const void *k, const void *v, void *out, void *out_low, float *lse, const int64_t *strides, uint32_t B, uint32_t Tq, uint32_t Tk,
                              uint32_t Hq, uint32_t Hk, uint32_t D, int32_t left, int32_t right, int32_t sinks, int32_t q_start, const int32_t *lengths, float scale,
                              int dtype, gfpp_stream_t stream);
+/* (cond_encoder.py:146-180, as above) */
+int gfpp_window_attn_two_part(uint32_t Tk, int32_t left, int32_t right, int32_t sinks, int dtype);
 /* Its backward pass (cond_encoder.py:146-180, as above): dq, dk, dv from dout, the forward pass' inputs, out and lse.  strides: {B, T, H} of q, k, v, out, dout, dq,
  * dk, dv.  Every row of dq, dk and dv is written (zeros behind a sequence's length).  No atomics: the same bits every time. */
-int gfpp_window_attn_backward(const void *q, const void *k, const void *v, const void *out, const void *dout, const float *lse, void *dq, void *dk, void *dv,
+int gfpp_window_attn_backward(const void *q, const void *k, const void *v, const void *out, const void *out_low, const void *dout, const float *lse, void *dq, void *dk, void *dv,
                               float *scratch, const int64_t *strides, uint32_t B, uint32_t Tq, uint32_t Tk, uint32_t Hq, uint32_t Hk, uint32_t D, int32_t left,
                               int32_t right, int32_t sinks, int32_t q_start, const int32_t *lengths, float scale, int dtype, gfpp_stream_t stream);
 /* (cond_encoder.py:146-180, as above) */
