@@ -498,7 +498,7 @@ __device__ __forceinline__ void lp_fill_shared(LpShared &sh, const LpTripArgs &a
 template <int AMB_D, typename H, bool SLOW, bool PROF = false>
 __global__ __launch_bounds__(kLpThreads, kLpThreads / 256) void k_head_trip_pool(LpTripArgs a) {
     __shared__ LpShared sh;
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);      // (in a scalar register: no vector register is spare across the blocks)
     constexpr bool prof = PROF;
     bool weights_resident = false;
     uint32_t barriers = 0;

@@ -9,7 +9,7 @@ name=$1; src=$2; shift 2
 cd "$(dirname "$0")/../genefaceplusplus_amd/csrc"
 make -s
 tmp=$(mktemp -d)
-/opt/rocm/bin/hipcc --offload-arch=gfx950 -O3 -std=c++17 -fPIC -ffp-contract=off -fvisibility=hidden -Wall -Wno-unused-function "$@" -c "$src" -o "$tmp/variant.o"
+/opt/rocm/bin/hipcc --offload-arch=gfx950 -O3 -std=c++17 -fPIC -ffp-contract=off -fvisibility=hidden -Wall -Wno-unused-function -Xclang -target-feature -Xclang -packed-fp32-ops "$@" -c "$src" -o "$tmp/variant.o"
 objs=$(ls *.o | grep -v "^${src%.hip}.o$")
 /opt/rocm/bin/hipcc --offload-arch=gfx950 -shared -fPIC -o "../../build/variants/lib_${name}.so" $objs "$tmp/variant.o"
 rm -rf "$tmp"
