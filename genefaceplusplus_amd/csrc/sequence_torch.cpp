@@ -299,7 +299,7 @@ struct WindowAttentionFn : torch::autograd::Function<WindowAttentionFn> {
         const Tensor dq = at::empty(q.sizes(), q.options()), dk = at::empty(k.sizes(), k.options()), dv = at::empty(v.sizes(), v.options());
         const auto w = ctx->saved_data["window"].toIntVector();
         const uint32_t B = (uint32_t)q.size(0), Tq = (uint32_t)q.size(1), Tk = (uint32_t)k.size(1), Hq = (uint32_t)q.size(2), Hk = (uint32_t)k.size(2), D = (uint32_t)q.size(3);
-        const Tensor scratch = at::empty({(int64_t)api.window_scratch(B, Tq, Tk, Hq, Hk, D, (int32_t)w[0], (int32_t)w[2], (int32_t)w[3])}, lse.options());
+        const Tensor scratch = at::empty({(int64_t)api.window_scratch(B, Tq, Tk, Hq, Hk, D, (int32_t)w[0], (int32_t)w[1], (int32_t)w[2], (int32_t)w[3], type_code("window_attention", q))}, lse.options());
         int64_t strides[24], *s = strides;
         for (const Tensor *t : {&q, &k, &v, &out, &dout, &dq, &dk, &dv}) put_strides(s, *t);
         check(api.window_backward(q.const_data_ptr(), k.const_data_ptr(), v.const_data_ptr(), out.const_data_ptr(), ptr(low), dout.const_data_ptr(), lse.const_data_ptr<float>(),

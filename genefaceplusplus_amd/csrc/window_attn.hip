@@ -15,15 +15,22 @@ namespace gfpp {
 template <typename T, int DP>
 constexpr int wa_bn() { return sizeof(T) == 4 && DP == 128 ? 32 : 64; }
 
-// TWO: probabilities as a rounded value and its remainder (window_attn_device.h: wa_two_part)
-template <typename T, int DP, bool VEC, bool TWO>
-__global__ __launch_bounds__(kWaThreads, sizeof(T) == 2 ? 2 : 1) void k_window_attn(WaArgs a) {
+// TWO: probabilities as a rounded value and its remainder (window_attn_device.h: wa_two_part).  HEADS 2: eight wavefronts, four for each of two query heads of a
+// group, share the tiles of keys and values -- half the loads and LDS writes per query.
+template <typename T, int DP, bool VEC, bool TWO, int HEADS>
+__global__ __launch_bounds__(kWaThreads * HEADS, sizeof(T) == 2 ? (DP <= 64 && VEC ? 3 : (VEC || HEADS == 2 ? 2 : 1)) : 1) void k_window_attn(WaArgs a) {
     constexpr int BN = wa_bn<T, DP>(), NS = DP / 16, NT = DP / 32, NSUB = BN / 32, PK = wa_pitch_row<T, DP>(), PV = wa_pitch_col<T, DP>();
     typedef typename LpTraits<T>::vec vec;
     __shared__ __attribute__((aligned(16))) unsigned char s_k[2][BN * PK], s_v[2][BN * PV];
     const int q_tiles = (a.Tq + kWaRows - 1) / kWaRows;
-    const int hq = (int)(blockIdx.x / q_tiles) % a.Hq, b = (int)(blockIdx.x / q_tiles) / a.Hq, i0 = (int)(blockIdx.x % q_tiles) * kWaRows, hk = hq / a.G;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = lane & 31, h = lane >> 5;
+    // items: sequence, key head, tile of queries, query head of the group -- those that read the same keys side by side
+    uint32_t item = wa_item(blockIdx.x, gridDim.x);
+    const int in_group = (int)(item % (a.G / HEADS)) * HEADS + (HEADS == 2 ? __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 8)) : 0);
+    item /= a.G / HEADS;
+    const int i0 = (int)(item % q_tiles) * kWaRows;
+    item /= q_tiles;
+    const int hk = (int)(item % a.Hk), hq = hk * a.G + in_group, b = (int)(item / a.Hk);
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6) & 3), c = lane & 31, h = lane >> 5;
     const int n = a.lengths ? a.lengths[b] < a.Tk ? a.lengths[b] : a.Tk : a.Tk;
     const int i = i0 + wave * 32 + c, p = a.q_start + i;
     const bool have = i < a.Tq && p < n;
@@ -41,7 +48,7 @@ __global__ __launch_bounds__(kWaThreads, sizeof(T) == 2 ? 2 : 1) void k_window_a
         for (int r = 0; r < 16; ++r) acc[t][r] = 0.0f;
     float m = -INFINITY, l = 0.0f;
     const T *kb = static_cast<const T *>(a.k.p) + b * a.k.sb + hk * a.k.sh, *vb = static_cast<const T *>(a.v.p) + b * a.v.sb + hk * a.v.sh;
-    WaStage<T, DP, BN, VEC> rk, rv;
+    WaStage<T, DP, BN, VEC, kWaThreads * HEADS> rk, rv;
     auto tile_row = [&](int k) { return (k < range.head ? k : range.lo + k - range.head) * BN; };
     if (tiles > 0) {
         rk.load(kb, a.k.st, tile_row(0), n, a.D);
@@ -70,12 +77,18 @@ __global__ __launch_bounds__(kWaThreads, sizeof(T) == 2 ? 2 : 1) void k_window_a
         if (seen) {
             v16f s[NSUB];
 #pragma unroll
-            for (int u = 0; u < NSUB; ++u) {
+            for (int u = 0; u < NSUB; ++u)
 #pragma unroll
                 for (int r = 0; r < 16; ++r) s[u][r] = 0.0f;
-#pragma unroll
-                for (int x = 0; x < NS; ++x) s[u] = LpTraits<T>::mfma(wa_row<T>(s_k[buf] + row_at + 32 * u * PK, x), q[x], s[u]);
+            {
+                WaStream<T, NSUB * NS> keys;
+                const auto read = [&](int x) { return wa_row<T>(s_k[buf] + row_at + 32 * (x / NS) * PK, x % NS); };
+                keys.prime(read);
+                keys.run(read, [&](int x, const vec &f) { s[x / NS] = LpTraits<T>::mfma(f, q[x % NS], s[x / NS]); });
             }
+            WaStream<T, NSUB * 2 * NT> values;                 // (32 keys u, their step x, the feature tile t: u, x, t)
+            const auto read_v = [&](int x) { return wa_col<T, PV>(s_v[buf] + col_at, 32 * (x / (2 * NT)) + 16 * (x / NT % 2), x % NT); };
+            values.prime(read_v);
             const bool full = pw1 < n && j1 < n && j1 <= pw0 + a.right && (j0 >= pw1 - a.left || j1 < a.sinks);
             if (!full) {
 #pragma unroll
@@ -110,21 +123,28 @@ __global__ __launch_bounds__(kWaThreads, sizeof(T) == 2 ? 2 : 1) void k_window_a
                     s[u][r] = wa_prob<TWO || sizeof(T) == 4>(s[u][r], top0, base, a.c);
                     l += s[u][r];
                 }
+            vec pr;
+            values.run(read_v, [&](int x, const vec &f) {
+                const int u = x / (2 * NT), step = x / NT % 2, t = x % NT;
+                if (t == 0) pr = wa_pack<T>(s[u], step);
+                acc[t] = LpTraits<T>::mfma(f, pr, acc[t]);
+            });
+            if constexpr (TWO) {                               // what the rounding left, over the same values once more
 #pragma unroll
-            for (int u = 0; u < NSUB; ++u)
+                for (int u = 0; u < NSUB; ++u)
 #pragma unroll
-                for (int x = 0; x < 2; ++x) {
-                    const vec pr = wa_pack<T>(s[u], x);
+                    for (int x = 0; x < 2; ++x) {
+                        const vec p = wa_pack<T>(s[u], x);
 #pragma unroll
-                    for (int t = 0; t < NT; ++t) acc[t] = LpTraits<T>::mfma(wa_col<T, PV>(s_v[buf] + col_at, 32 * u + 16 * x, t), pr, acc[t]);
-                    if constexpr (TWO) {
-#pragma unroll
-                        for (int e = 0; e < 8; ++e) s[u][8 * x + e] -= (float)pr[e];
-                        const vec rest = wa_pack<T>(s[u], x);
-#pragma unroll
-                        for (int t = 0; t < NT; ++t) acc[t] = LpTraits<T>::mfma(wa_col<T, PV>(s_v[buf] + col_at, 32 * u + 16 * x, t), rest, acc[t]);
+                        for (int e = 0; e < 8; ++e) s[u][8 * x + e] -= (float)p[e];
                     }
-                }
+                values.prime(read_v);
+                values.run(read_v, [&](int x, const vec &f) {
+                    const int u = x / (2 * NT), step = x / NT % 2, t = x % NT;
+                    if (t == 0) pr = wa_pack<T>(s[u], step);
+                    acc[t] = LpTraits<T>::mfma(f, pr, acc[t]);
+                });
+            }
         }
         __syncthreads();
     }
@@ -139,8 +159,9 @@ __global__ __launch_bounds__(kWaThreads, sizeof(T) == 2 ? 2 : 1) void k_window_a
     if (a.lse && h == 0) a.lse[((int64_t)b * a.Hq + hq) * a.Tq + i] = l > 0.0f ? m * a.c + log2f(l) : INFINITY;
 }
 
+// whether a tensor's rows can be read as 16-byte vectors whose place in a tile of 64 rows is a 32-bit offset (WaStage)
 bool wa_vectors(const WaTensor &t, int D, size_t size) {
-    return ((uintptr_t)t.p | (uint64_t)(t.sb * (int64_t)size) | (uint64_t)(t.st * (int64_t)size) | (uint64_t)(t.sh * (int64_t)size) | (uint64_t)(D * size)) % 16 == 0;
+    return t.st >= D && t.st <= (int64_t)(((1u << 31) - 1024) / (64 * size)) && ((uintptr_t)t.p | (uint64_t)(t.sb * (int64_t)size) | (uint64_t)(t.st * (int64_t)size) | (uint64_t)(t.sh * (int64_t)size) | (uint64_t)(D * size)) % 16 == 0;
 }
 
 // the arguments that both passes share; 0 or an error code
@@ -186,11 +207,19 @@ int wa_arguments(const char *what, WaArgs &a, const int64_t *strides, int n_tens
     return 0;
 }
 
+template <typename T, int DP, bool TWO, int HEADS>
+static void wa_forward_launch(const WaArgs &a, bool vec, uint32_t grid, hipStream_t st) {
+    if (vec) k_window_attn<T, DP, true, TWO, HEADS><<<grid / HEADS, kWaThreads * HEADS, 0, st>>>(a);
+    else k_window_attn<T, DP, false, TWO, HEADS><<<grid / HEADS, kWaThreads * HEADS, 0, st>>>(a);
+}
 template <typename T, bool TWO>
 static void wa_forward(const WaArgs &a, bool vec, uint32_t grid, hipStream_t st) {
-    if (a.D <= 32) vec ? k_window_attn<T, 32, true, TWO><<<grid, kWaThreads, 0, st>>>(a) : k_window_attn<T, 32, false, TWO><<<grid, kWaThreads, 0, st>>>(a);
-    else if (a.D <= 64) vec ? k_window_attn<T, 64, true, TWO><<<grid, kWaThreads, 0, st>>>(a) : k_window_attn<T, 64, false, TWO><<<grid, kWaThreads, 0, st>>>(a);
-    else vec ? k_window_attn<T, 128, true, TWO><<<grid, kWaThreads, 0, st>>>(a) : k_window_attn<T, 128, false, TWO><<<grid, kWaThreads, 0, st>>>(a);
+    if (a.D <= 32) wa_forward_launch<T, 32, TWO, 1>(a, vec, grid, st);
+    else if (a.D <= 64) wa_forward_launch<T, 64, TWO, 1>(a, vec, grid, st);
+    else if constexpr (sizeof(T) == 2 && !TWO) {
+        if (vec && wa_pair_heads(a, grid)) k_window_attn<T, 128, true, TWO, 2><<<grid / 2, kWaThreads * 2, 0, st>>>(a);
+        else wa_forward_launch<T, 128, TWO, 1>(a, vec, grid, st);
+    } else wa_forward_launch<T, 128, TWO, 1>(a, vec, grid, st);
 }
 
 }  // namespace gfpp

@@ -16,14 +16,21 @@ int wa_arguments(const char *what, WaArgs &a, const int64_t *strides, int n_tens
                  int32_t right, int32_t sinks, int32_t q_start, const int32_t *lengths, float scale, int dtype);
 bool wa_vectors(const WaTensor &t, int D, size_t size);
 
-template <typename T, int DP, bool VEC>
-__global__ __launch_bounds__(kWaThreads, sizeof(T) == 2 ? 2 : 1) void k_window_attn_dq(WaArgs a) {
+// (HEADS: as in the forward pass)
+template <typename T, int DP, bool VEC, int HEADS>
+__global__ __launch_bounds__(kWaThreads * HEADS, sizeof(T) == 2 && (VEC || DP <= 64) ? 2 : 1) void k_window_attn_dq(WaArgs a) {
     constexpr int BN = sizeof(T) == 4 && DP == 128 ? 32 : 64, NS = DP / 16, NT = DP / 32, PK = wa_pitch_both<T, DP>(), PV = wa_pitch_row<T, DP>();
     typedef typename LpTraits<T>::vec vec;
     __shared__ __attribute__((aligned(16))) unsigned char s_k[2][BN * PK], s_v[2][BN * PV];
     const int q_tiles = (a.Tq + kWaRows - 1) / kWaRows;
-    const int hq = (int)(blockIdx.x / q_tiles) % a.Hq, b = (int)(blockIdx.x / q_tiles) / a.Hq, i0 = (int)(blockIdx.x % q_tiles) * kWaRows, hk = hq / a.G;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = lane & 31, h = lane >> 5;
+    // items: sequence, key head, tile of queries, query head of the group -- those that read the same keys side by side
+    uint32_t item = wa_item(blockIdx.x, gridDim.x);
+    const int in_group = (int)(item % (a.G / HEADS)) * HEADS + (HEADS == 2 ? __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 8)) : 0);
+    item /= a.G / HEADS;
+    const int i0 = (int)(item % q_tiles) * kWaRows;
+    item /= q_tiles;
+    const int hk = (int)(item % a.Hk), hq = hk * a.G + in_group, b = (int)(item / a.Hk);
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6) & 3), c = lane & 31, h = lane >> 5;
     const int n = a.lengths ? a.lengths[b] < a.Tk ? a.lengths[b] : a.Tk : a.Tk;
     const int i = i0 + wave * 32 + c, p = a.q_start + i;
     const bool have = i < a.Tq && p < n;                       // (rows behind the sequence: zeros, whatever they hold)
@@ -64,7 +71,7 @@ __global__ __launch_bounds__(kWaThreads, sizeof(T) == 2 ? 2 : 1) void k_window_a
 #pragma unroll
         for (int r = 0; r < 16; ++r) acc[t][r] = 0.0f;
     const T *kb = static_cast<const T *>(a.k.p) + b * a.k.sb + hk * a.k.sh, *vb = static_cast<const T *>(a.v.p) + b * a.v.sb + hk * a.v.sh;
-    WaStage<T, DP, BN, VEC> rk, rv;
+    WaStage<T, DP, BN, VEC, kWaThreads * HEADS> rk, rv;
     auto tile_row = [&](int k) { return (k < range.head ? k : range.lo + k - range.head) * BN; };
     if (tiles > 0) {
         rk.load(kb, a.k.st, tile_row(0), n, a.D);
@@ -93,76 +100,83 @@ __global__ __launch_bounds__(kWaThreads, sizeof(T) == 2 ? 2 : 1) void k_window_a
         const bool seen = pw0 < n && j0 <= pw1 + a.right && (j1 >= pw0 - a.left || j0 < a.sinks);
         if (seen) {
             const bool full = pw1 < n && j1 < n && j1 <= pw0 + a.right && (j0 >= pw1 - a.left || j1 < a.sinks);
-            // Two bodies without a branch inside: the products of one half tile may then overlap the arithmetic of the other.  The widest heads have no registers
-            // for two half tiles at once (two wavefronts per SIMD overlap instead): one body, the branch between its products.
-            auto body = [&](auto masked, auto always) {
 #pragma unroll
-                for (int u = 0; u < BN / 32; ++u) {
-                    v16f s, d;
+            for (int u = 0; u < BN / 32; ++u) {
+                v16f s, d;
 #pragma unroll
-                    for (int r = 0; r < 16; ++r) s[r] = d[r] = 0.0f;
+                for (int r = 0; r < 16; ++r) s[r] = d[r] = 0.0f;
+                {
+                    WaStream<T, 2 * NS> rows;                  // keys, then values
+                    const auto read = [&](int x) { return x < NS ? wa_row<T>(s_k[buf] + row_k + 32 * u * PK, x) : wa_row<T>(s_v[buf] + row_v + 32 * u * PV, x - NS); };
+                    rows.prime(read);
+                    rows.run(read, [&](int x, const vec &f) {
+                        if (x < NS) s = LpTraits<T>::mfma(f, q[x % NS], s);
+                        else d = LpTraits<T>::mfma(f, g[x % NS], d);
+                    });
+                }
+                WaStream<T, 2 * NT> cols;
+                const auto read_k = [&](int x) { return wa_col<T, PK>(s_k[buf] + col_at, 32 * u + 16 * (x / NT), x % NT); };
+                cols.prime(read_k);
+                if (!full) {
 #pragma unroll
-                    for (int x = 0; x < NS; ++x) s = LpTraits<T>::mfma(wa_row<T>(s_k[buf] + row_k + 32 * u * PK, x), q[x], s);
-#pragma unroll
-                    for (int x = 0; x < NS; ++x) d = LpTraits<T>::mfma(wa_row<T>(s_v[buf] + row_v + 32 * u * PV, x), g[x], d);
-                    if (decltype(masked)::value && (decltype(always)::value || !full)) {
-#pragma unroll
-                        for (int r = 0; r < 16; ++r) {
-                            const int j = j0 + 32 * u + 8 * (r >> 2) + 4 * h + (r & 3);
-                            s[r] = j <= last && (j >= first || j < a.sinks) ? s[r] : -INFINITY;
-                        }
-                    }
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], a.c, -lse)) * (d[r] - delta);
-#pragma unroll
-                    for (int x = 0; x < 2; ++x) {
-                        const vec ds = wa_pack<T>(s, x);
-#pragma unroll
-                        for (int t = 0; t < NT; ++t) acc[t] = LpTraits<T>::mfma(wa_col<T, PK>(s_k[buf] + col_at, 32 * u + 16 * x, t), ds, acc[t]);
+                    for (int r = 0; r < 16; ++r) {
+                        const int j = j0 + 32 * u + 8 * (r >> 2) + 4 * h + (r & 3);
+                        s[r] = j <= last && (j >= first || j < a.sinks) ? s[r] : -INFINITY;
                     }
                 }
-            };
-            if constexpr (DP == 128) body(WaFlag<true>{}, WaFlag<false>{});
-            else if (full) body(WaFlag<false>{}, WaFlag<false>{});
-            else body(WaFlag<true>{}, WaFlag<true>{});
+#pragma unroll
+                for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], a.c, -lse)) * (d[r] - delta);
+                vec ds;
+                cols.run(read_k, [&](int x, const vec &f) {
+                    if (x % NT == 0) ds = wa_pack<T>(s, x / NT);
+                    acc[x % NT] = LpTraits<T>::mfma(f, ds, acc[x % NT]);
+                });
+            }
         }
         __syncthreads();
     }
     if (i < a.Tq) wa_store_rows<T, NT, VEC>(acc, a.scale, static_cast<T *>(a.dq.p) + b * a.dq.sb + (int64_t)i * a.dq.st + hq * a.dq.sh, h, a.D);
 }
 
-// dk and dv of 128 keys (a wavefront: 32), the queries in tiles of BQ through LDS.  Work items: first the slices of the tiles with sinks (a.splits each, partial
-// sums), then the other tiles.
-template <typename T, int DP, bool VEC>
-__global__ __launch_bounds__(kWaThreads, 1) void k_window_attn_dkv(WaArgs a) {
-    constexpr int BQ = sizeof(T) == 2 ? 64 : 32, NS = DP / 16, NT = DP / 32, PITCH = wa_pitch_both<T, DP>();
+// dk and dv of 128 (64) keys, the queries in tiles of 32 through LDS.  Two wavefronts for every 32 keys: one makes the probabilities and sums dv, the other takes
+// them a tile later (through LDS, in fp32), makes ds and sums dk.  One wavefront doing both would hold 128 accumulators, 64 registers of K and V and both products:
+// alone on its SIMD, 23 % of the matrix pipe's cycles were used.  Halved, two or more share a SIMD and fill each other's waits; the work is the same (four
+// products per tile, none twice).  Three tiles are held: the one being stored, the one that is read by the first wavefronts and the one that is read by the second.
+// Work items: first the slices of the tiles with sinks (a.splits each, partial sums), then the other tiles.
+// PAIRS: of wavefronts, 32 keys each: 4, or 2 where 128 keys a workgroup would leave CUs without one (and for the widest fp32 heads, which need the registers).
+constexpr int kWaBq = 32;
+template <typename T, int DP, bool VEC, int PAIRS>
+__global__ __launch_bounds__(PAIRS * 128, sizeof(T) == 4 && DP == 128 ? 1 : 2) void k_window_attn_dkv(WaArgs a) {
+    constexpr int KEYS = PAIRS * 32, BQ = kWaBq, NS = DP / 16, NT = DP / 32, PITCH = wa_pitch_both<T, DP>();
     typedef typename LpTraits<T>::vec vec;
     typedef float f4 __attribute__((ext_vector_type(4)));
-    __shared__ __attribute__((aligned(16))) unsigned char s_q[2][BQ * PITCH], s_g[2][BQ * PITCH];
-    __shared__ __attribute__((aligned(16))) float s_lse[2][BQ], s_delta[2][BQ];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = lane & 31, h = lane >> 5;
+    __shared__ __attribute__((aligned(16))) unsigned char s_q[3][BQ * PITCH], s_g[3][BQ * PITCH];
+    __shared__ __attribute__((aligned(16))) float s_p[2][PAIRS][4][64][4];                 // [tile & 1][32 keys][quad of rows][lane][row]
+    __shared__ __attribute__((aligned(16))) float s_lse[3][BQ], s_delta[3][BQ];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)), keys = wave % PAIRS, c = lane & 31, h = lane >> 5;
+    const bool second = wave >= PAIRS;
     const uint32_t bh = (uint32_t)a.B * a.Hk, sliced = a.sink_tiles * a.splits * bh;
     const bool slice = blockIdx.x < sliced;
-    uint32_t item = slice ? blockIdx.x : blockIdx.x - sliced;
-    const uint32_t hkb = item % bh;
-    item /= bh;
+    uint32_t item = slice ? blockIdx.x : wa_item(blockIdx.x - sliced, gridDim.x - sliced);
+    const uint32_t per_head = slice ? a.sink_tiles * a.splits : (gridDim.x - sliced) / bh, hkb = item / per_head;
+    item %= per_head;
     const uint32_t part = slice ? item % a.splits : 0;
-    const int j0 = (int)(slice ? item / a.splits : item + a.sink_tiles) * kWaRows;
+    const int j0 = (int)(slice ? item / a.splits : item + a.sink_tiles) * KEYS;
     const int hk = (int)(hkb % a.Hk), b = (int)(hkb / a.Hk);
     const int n = a.lengths ? a.lengths[b] < a.Tk ? a.lengths[b] : a.Tk : a.Tk;
-    const int j = j0 + wave * 32 + c, jw0 = j0 + wave * 32, jw1 = jw0 + 31;
+    const int jw0 = j0 + keys * 32, jw1 = jw0 + 31, j = jw0 + c;
     const bool have = j < n;
-    vec kf[NS], vf[NS];
-    wa_global_rows<T, NS, VEC>(kf, static_cast<const T *>(a.k.p) + b * a.k.sb + (int64_t)j * a.k.st + hk * a.k.sh, have, h, a.D);
-    wa_global_rows<T, NS, VEC>(vf, static_cast<const T *>(a.v.p) + b * a.v.sb + (int64_t)j * a.v.st + hk * a.v.sh, have, h, a.D);
-    v16f dk[NT], dv[NT];
+    vec f[NS];                                                                         // the lane's key (first) or value (second)
+    const WaTensor &own = second ? a.v : a.k;
+    wa_global_rows<T, NS, VEC>(f, static_cast<const T *>(own.p) + b * own.sb + (int64_t)j * own.st + hk * own.sh, have, h, a.D);
+    v16f acc[NT];                                                                      // dv (first) or dk (second)
 #pragma unroll
     for (int t = 0; t < NT; ++t)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) dk[t][r] = dv[t][r] = 0.0f;
+        for (int r = 0; r < 16; ++r) acc[t][r] = 0.0f;
     // query rows [i_lo, i_hi) that can see a key of the tile; rows from `end` on are behind the sequence
     const int end = n - a.q_start < a.Tq ? n - a.q_start : a.Tq;
-    const int jn = j0 + kWaRows <= n ? j0 + kWaRows - 1 : n - 1;
+    const int jn = j0 + KEYS <= n ? j0 + KEYS - 1 : n - 1;
     int i_lo = j0 - a.right - a.q_start, i_hi = (j0 < a.sinks ? end : jn + a.left + 1 - a.q_start);
     i_lo = i_lo < 0 ? 0 : i_lo / BQ * BQ;
     i_hi = i_hi < end ? i_hi : end;
@@ -175,10 +189,11 @@ __global__ __launch_bounds__(kWaThreads, 1) void k_window_attn_dkv(WaArgs a) {
         tiles = tiles < 0 ? 0 : tiles;
     }
     const int steps = tiles * a.G;
-    WaStage<T, DP, BQ, VEC> rq, rg;
+    WaStage<T, DP, BQ, VEC, PAIRS * 128> rq, rg;
     float r_stat = 0.0f;
-    auto load = [&](int s) {
-        const int hq = hk * a.G + s / tiles, i = i_lo + s % tiles * BQ;
+    int next_tile = 0, next_head = 0;                                                  // of the tile that is loaded next: the heads of a group one after the other
+    auto load = [&]() {
+        const int hq = hk * a.G + next_head, i = i_lo + next_tile * BQ;
         rq.load(static_cast<const T *>(a.q.p) + b * a.q.sb + hq * a.q.sh, a.q.st, i, end, a.D);
         rg.load(static_cast<const T *>(a.dout.p) + b * a.dout.sb + hq * a.dout.sh, a.dout.st, i, end, a.D);
         if (threadIdx.x < 2 * BQ) {
@@ -186,6 +201,10 @@ __global__ __launch_bounds__(kWaThreads, 1) void k_window_attn_dkv(WaArgs a) {
             const int64_t at = ((int64_t)b * a.Hq + hq) * a.Tq + row;
             if (threadIdx.x < BQ) r_stat = row < end ? a.lse[at] : INFINITY;
             else r_stat = row < end ? a.delta[at] : 0.0f;
+        }
+        if (++next_tile == tiles) {
+            next_tile = 0;
+            ++next_head;
         }
     };
     auto store = [&](int buf) {
@@ -195,75 +214,96 @@ __global__ __launch_bounds__(kWaThreads, 1) void k_window_attn_dkv(WaArgs a) {
         else if (threadIdx.x < 2 * BQ) s_delta[buf][threadIdx.x - BQ] = r_stat;
     };
     if (steps > 0) {
-        load(0);
+        load();
         store(0);
-        if (steps > 1) load(1);
+        if (steps > 1) load();
     }
-    wa_arrived(kf);
-    wa_arrived(vf);
+    wa_arrived(f);
     __syncthreads();
     const int row_at = c * PITCH + 8 * h * (int)sizeof(T), col_at = wa_col_offset<T>(lane, PITCH);
-    for (int k = 0; k < steps; ++k) {
-        const int buf = k & 1, p0 = a.q_start + i_lo + k % tiles * BQ, p1 = p0 + BQ - 1;
+    const int from = have ? j - a.right : 0x7fffffff, to = j < a.sinks ? 0x7fffffff : j + a.left;
+    int now = 0, tile = second ? -1 : 0, buf = second ? 2 : 0;                         // buffer of step k; this wavefront's tile and its buffer (one step behind: second)
+    for (int k = 0; k <= steps; ++k) {
+        const int next = now == 2 ? 0 : now + 1;
         if (k + 1 < steps) {
-            store(buf ^ 1);
-            if (k + 2 < steps) load(k + 2);
+            store(next);                                                               // (tile k - 2's: last read a step ago, before the barrier)
+            if (k + 2 < steps) load();
         }
+        const int p0 = a.q_start + i_lo + tile * BQ, p1 = p0 + BQ - 1;
         const bool seen = jw0 < n && p1 >= jw0 - a.right && (p0 <= jw1 + a.left || jw0 < a.sinks);
-        if (seen) {
-            const bool full = jw1 < n && p0 >= jw1 - a.right && (p1 <= jw0 + a.left || jw1 < a.sinks);
-            // (two bodies without a branch inside: the compiler overlaps the products of one sub-tile with the arithmetic of the other)
-            auto body = [&](auto masked) {
+        if (!second) {
+            if (k < steps && seen) {
+                v16f s;
 #pragma unroll
-                for (int u = 0; u < BQ / 32; ++u) {
-                    v16f s, d;
+                for (int r = 0; r < 16; ++r) s[r] = 0.0f;
+                {
+                    WaStream<T, NS> rows;
+                    const auto read = [&](int x) { return wa_row<T>(s_q[buf] + row_at, x); };
+                    rows.prime(read);
+                    rows.run(read, [&](int x, const vec &y) { s = LpTraits<T>::mfma(y, f[x], s); });
+                }
+                WaStream<T, 2 * NT> cols;
+                const auto read_g = [&](int x) { return wa_col<T, PITCH>(s_g[buf] + col_at, 16 * (x / NT), x % NT); };
+                cols.prime(read_g);
+                if (!(jw1 < n && p0 >= jw1 - a.right && (p1 <= jw0 + a.left || jw1 < a.sinks))) {
 #pragma unroll
-                    for (int r = 0; r < 16; ++r) s[r] = d[r] = 0.0f;
-#pragma unroll
-                    for (int x = 0; x < NS; ++x) s = LpTraits<T>::mfma(wa_row<T>(s_q[buf] + row_at + 32 * u * PITCH, x), kf[x], s);
-#pragma unroll
-                    for (int x = 0; x < NS; ++x) d = LpTraits<T>::mfma(wa_row<T>(s_g[buf] + row_at + 32 * u * PITCH, x), vf[x], d);
-                    if constexpr (decltype(masked)::value) {
-                        const int from = have ? j - a.right : 0x7fffffff, to = j < a.sinks ? 0x7fffffff : j + a.left;
-#pragma unroll
-                        for (int r = 0; r < 16; ++r) {
-                            const int p = p0 + 32 * u + 8 * (r >> 2) + 4 * h + (r & 3);
-                            s[r] = p >= from && p <= to ? s[r] : -INFINITY;
-                        }
-                    }
-#pragma unroll
-                    for (int r = 0; r < 16; r += 4) {
-                        const f4 lse = *reinterpret_cast<const f4 *>(&s_lse[buf][32 * u + 2 * r + 4 * h]), delta = *reinterpret_cast<const f4 *>(&s_delta[buf][32 * u + 2 * r + 4 * h]);
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            s[r + e] = __builtin_amdgcn_exp2f(fmaf(s[r + e], a.c, -lse[e]));
-                            d[r + e] = s[r + e] * (d[r + e] - delta[e]);
-                        }
-                    }
-#pragma unroll
-                    for (int x = 0; x < 2; ++x) {
-                        const vec pr = wa_pack<T>(s, x), ds = wa_pack<T>(d, x);
-#pragma unroll
-                        for (int t = 0; t < NT; ++t) {
-                            dv[t] = LpTraits<T>::mfma(wa_col<T, PITCH>(s_g[buf] + col_at, 32 * u + 16 * x, t), pr, dv[t]);
-                            dk[t] = LpTraits<T>::mfma(wa_col<T, PITCH>(s_q[buf] + col_at, 32 * u + 16 * x, t), ds, dk[t]);
-                        }
+                    for (int r = 0; r < 16; ++r) {
+                        const int p = p0 + 8 * (r >> 2) + 4 * h + (r & 3);
+                        s[r] = p >= from && p <= to ? s[r] : -INFINITY;
                     }
                 }
-            };
-            if (full) body(WaFlag<false>{});
-            else body(WaFlag<true>{});
+#pragma unroll
+                for (int r = 0; r < 16; r += 4) {
+                    const f4 lse = *reinterpret_cast<const f4 *>(&s_lse[buf][2 * r + 4 * h]);
+                    f4 pr;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) pr[e] = s[r + e] = __builtin_amdgcn_exp2f(fmaf(s[r + e], a.c, -lse[e]));
+                    *reinterpret_cast<f4 *>(s_p[k & 1][keys][r >> 2][lane]) = pr;
+                }
+                vec pr;
+                cols.run(read_g, [&](int x, const vec &y) {
+                    if (x % NT == 0) pr = wa_pack<T>(s, x / NT);
+                    acc[x % NT] = LpTraits<T>::mfma(y, pr, acc[x % NT]);
+                });
+            }
+        } else if (k > 0 && seen) {
+            v16f d;
+#pragma unroll
+            for (int r = 0; r < 16; ++r) d[r] = 0.0f;
+            {
+                WaStream<T, NS> rows;
+                const auto read = [&](int x) { return wa_row<T>(s_g[buf] + row_at, x); };
+                rows.prime(read);
+                rows.run(read, [&](int x, const vec &y) { d = LpTraits<T>::mfma(y, f[x], d); });
+            }
+            WaStream<T, 2 * NT> cols;
+            const auto read_q = [&](int x) { return wa_col<T, PITCH>(s_q[buf] + col_at, 16 * (x / NT), x % NT); };
+            cols.prime(read_q);
+#pragma unroll
+            for (int r = 0; r < 16; r += 4) {
+                const f4 delta = *reinterpret_cast<const f4 *>(&s_delta[buf][2 * r + 4 * h]), pr = *reinterpret_cast<const f4 *>(s_p[(k - 1) & 1][keys][r >> 2][lane]);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) d[r + e] = pr[e] * (d[r + e] - delta[e]);
+            }
+            vec ds;
+            cols.run(read_q, [&](int x, const vec &y) {
+                if (x % NT == 0) ds = wa_pack<T>(d, x / NT);
+                acc[x % NT] = LpTraits<T>::mfma(y, ds, acc[x % NT]);
+            });
         }
         __syncthreads();
+        now = next;
+        buf = buf == 2 ? 0 : buf + 1;
+        if (++tile == tiles) tile = 0;
     }
     if (j >= a.Tk) return;
+    const float f_out = second ? a.scale : 1.0f;
     if (slice) {
-        float *out = a.partial + ((((int64_t)(j0 / kWaRows) * a.splits + part) * bh + hkb) * 2 * kWaRows + (j - j0)) * a.D;
-        wa_store_rows<float, NT, false>(dk, a.scale, out, h, a.D);
-        wa_store_rows<float, NT, false>(dv, 1.0f, out + kWaRows * a.D, h, a.D);
+        float *out = a.partial + (((((int64_t)(j0 / KEYS) * a.splits + part) * bh + hkb) * 2 + (second ? 0 : 1)) * KEYS + (j - j0)) * a.D;
+        wa_store_rows<float, NT, false>(acc, f_out, out, h, a.D);
     } else {
-        wa_store_rows<T, NT, VEC>(dk, a.scale, static_cast<T *>(a.dk.p) + b * a.dk.sb + (int64_t)j * a.dk.st + hk * a.dk.sh, h, a.D);
-        wa_store_rows<T, NT, VEC>(dv, 1.0f, static_cast<T *>(a.dv.p) + b * a.dv.sb + (int64_t)j * a.dv.st + hk * a.dv.sh, h, a.D);
+        const WaTensor &o = second ? a.dk : a.dv;
+        wa_store_rows<T, NT, VEC>(acc, f_out, static_cast<T *>(o.p) + b * o.sb + (int64_t)j * o.st + hk * o.sh, h, a.D);
     }
 }
 
@@ -272,45 +312,59 @@ template <typename T>
 __global__ __launch_bounds__(kWaThreads) void k_window_attn_join(WaArgs a) {
     const uint32_t bh = (uint32_t)a.B * a.Hk, hkb = blockIdx.y, tile = blockIdx.z;
     const int hk = (int)(hkb % a.Hk), b = (int)(hkb / a.Hk);
-    const int64_t size = 2ll * kWaRows * a.D, stride = (int64_t)bh * size;
+    const int64_t size = 2ll * a.keys * a.D, stride = (int64_t)bh * size;
     const float *src = a.partial + ((int64_t)tile * a.splits * bh + hkb) * size;
     for (int64_t e = blockIdx.x * kWaThreads + threadIdx.x; e < size; e += (int64_t)gridDim.x * kWaThreads) {
-        const int which = e >= (int64_t)kWaRows * a.D, r = (int)(e / a.D) - which * kWaRows, d = (int)(e % a.D);
-        const int64_t j = (int64_t)tile * kWaRows + r;
+        const int which = e >= (int64_t)a.keys * a.D, r = (int)(e / a.D) - which * a.keys, d = (int)(e % a.D);
+        const int64_t j = (int64_t)tile * a.keys + r;
         if (j >= a.Tk) continue;
         float sum = 0.0f;
-        for (uint32_t s = 0; s < a.splits; ++s) sum += src[s * stride + e];
+        uint32_t s = 0;
+        for (; s + 8 <= a.splits; s += 8) {                    // (eight loads in flight; the order of the sum stays)
+            float v[8];
+#pragma unroll
+            for (int x = 0; x < 8; ++x) v[x] = src[(s + x) * stride + e];
+#pragma unroll
+            for (int x = 0; x < 8; ++x) sum += v[x];
+        }
+        for (; s < a.splits; ++s) sum += src[s * stride + e];
         const WaTensor &t = which ? a.dv : a.dk;
         static_cast<T *>(t.p)[b * t.sb + j * t.st + hk * t.sh + d] = (T)sum;
     }
 }
 
-// slices of a tile with sinks: enough for the chip, at least 512 queries each
-static uint32_t wa_splits(uint32_t sink_tiles, uint64_t bh, uint32_t Tq) {
-    if (sink_tiles == 0) return 1;
-    const uint64_t want = ((uint64_t)cu_count() + sink_tiles * bh - 1) / (sink_tiles * bh), most = Tq / 512;
-    const uint64_t n = want < most ? want : most;
-    return n < 1 ? 1 : (uint32_t)n;
+// slices of a tile with sinks: each about the queries that a tile without sinks has, so that no workgroup ends long after the others; at least 256, 64 slices at most
+static uint32_t wa_splits(const WaArgs &a) {
+    const int64_t ordinary = (int64_t)a.keys + a.left + a.right, each = ordinary > 256 ? ordinary : 256, want = ((int64_t)a.Tq + each - 1) / each;
+    return (uint32_t)(want < 1 ? 1 : (want > 64 ? 64 : want));
 }
 static uint32_t wa_sink_tiles(const WaArgs &a) {
     // a window that reaches every query from its first key makes the sinks ordinary keys
     if (a.sinks == 0 || (int64_t)a.left + 1 >= (int64_t)a.q_start + a.Tq) return 0;
-    return (uint32_t)(a.sinks + kWaRows - 1) / kWaRows;
+    return (uint32_t)((a.sinks + a.keys - 1) / a.keys);
 }
 
+template <typename T, int DP>
+static void wa_backward_launch(const WaArgs &a, bool vec, uint32_t gq, uint32_t gk, hipStream_t st) {
+    if (gq) {
+        bool paired = false;
+        if constexpr (sizeof(T) == 2 && DP == 128) {
+            paired = vec && wa_pair_heads(a, gq);
+            if (paired) k_window_attn_dq<T, DP, true, 2><<<gq / 2, kWaThreads * 2, 0, st>>>(a);
+        }
+        if (!paired) vec ? k_window_attn_dq<T, DP, true, 1><<<gq, kWaThreads, 0, st>>>(a) : k_window_attn_dq<T, DP, false, 1><<<gq, kWaThreads, 0, st>>>(a);
+    }
+    if (!gk) return;
+    if (a.keys == 64) vec ? k_window_attn_dkv<T, DP, true, 2><<<gk, 256, 0, st>>>(a) : k_window_attn_dkv<T, DP, false, 2><<<gk, 256, 0, st>>>(a);
+    if constexpr (sizeof(T) == 2 || DP < 128)
+        if (a.keys == 128) vec ? k_window_attn_dkv<T, DP, true, 4><<<gk, 512, 0, st>>>(a) : k_window_attn_dkv<T, DP, false, 4><<<gk, 512, 0, st>>>(a);
+    if (a.sink_tiles) k_window_attn_join<T><<<dim3(div_up(2 * a.keys * a.D, kWaThreads), (uint32_t)(a.B * a.Hk), a.sink_tiles), kWaThreads, 0, st>>>(a);
+}
 template <typename T>
 static void wa_backward(const WaArgs &a, bool vec, uint32_t gq, uint32_t gk, hipStream_t st) {
-#define WA_BOTH(DP)                                                                                                                    \
-    do {                                                                                                                               \
-        if (gq) vec ? k_window_attn_dq<T, DP, true><<<gq, kWaThreads, 0, st>>>(a) : k_window_attn_dq<T, DP, false><<<gq, kWaThreads, 0, st>>>(a);    \
-        if (gk) vec ? k_window_attn_dkv<T, DP, true><<<gk, kWaThreads, 0, st>>>(a) : k_window_attn_dkv<T, DP, false><<<gk, kWaThreads, 0, st>>>(a);  \
-    } while (0)
-    if (a.D <= 32) WA_BOTH(32);
-    else if (a.D <= 64) WA_BOTH(64);
-    else WA_BOTH(128);
-#undef WA_BOTH
-    if (a.sink_tiles && gk)
-        k_window_attn_join<T><<<dim3(div_up(2 * kWaRows * a.D, kWaThreads), (uint32_t)(a.B * a.Hk), a.sink_tiles), kWaThreads, 0, st>>>(a);
+    if (a.D <= 32) wa_backward_launch<T, 32>(a, vec, gq, gk, st);
+    else if (a.D <= 64) wa_backward_launch<T, 64>(a, vec, gq, gk, st);
+    else wa_backward_launch<T, 128>(a, vec, gq, gk, st);
 }
 
 }  // namespace gfpp
@@ -325,24 +379,33 @@ using namespace gfpp;
         }                                                              \
     } while (0)
 
-static void wa_bwd_setup(WaArgs &a) {
+// 128 keys a workgroup, or 64 where there would be fewer than two workgroups for every CU, and for fp32 heads over 64
+static int wa_bwd_keys(const WaArgs &a, int dtype) {
+    const uint64_t groups = (uint64_t)((a.Tk + 127) / 128) * a.B * a.Hk;
+    return groups < 2ull * cu_count() || (dtype == GFPP_F32 && a.D > 64) ? 64 : 128;
+}
+static void wa_bwd_setup(WaArgs &a, int dtype) {
+    a.keys = wa_bwd_keys(a, dtype);
     a.sink_tiles = wa_sink_tiles(a);
-    a.splits = wa_splits(a.sink_tiles, (uint64_t)a.B * a.Hk, (uint32_t)a.Tq);
+    a.splits = a.sink_tiles ? wa_splits(a) : 1;
     if (a.splits == 1) a.sink_tiles = 0;                       // whole tiles write their gradients themselves
 }
 
 GFPP_API unsigned long long gfpp_window_attn_backward_scratch_floats(uint32_t B, uint32_t Tq, uint32_t Tk, uint32_t Hq, uint32_t Hk, uint32_t D, int32_t left,
-                                                                     int32_t sinks, int32_t q_start) {
-    if (Hk == 0 || Tq > (1u << 29) || Tk > (1u << 29) || sinks < 0 || left < 0) return 0;
+                                                                     int32_t right, int32_t sinks, int32_t q_start, int dtype) {
+    if (Hk == 0 || Tq > (1u << 29) || Tk > (1u << 29) || sinks < 0 || left < 0 || right < 0) return 0;
     WaArgs a{};
     a.B = (int)B;
     a.Hk = (int)Hk;
     a.Tq = (int)Tq;
+    a.Tk = (int)Tk;
+    a.D = (int)D;
     a.left = left < (1 << 29) ? left : 1 << 29;                // (as wa_arguments has them)
+    a.right = right < (1 << 29) ? right : 1 << 29;
     a.sinks = sinks < (int)Tk ? sinks : (int)Tk;
     a.q_start = q_start;
-    wa_bwd_setup(a);
-    return (unsigned long long)B * Hq * Tq + (unsigned long long)a.sink_tiles * a.splits * B * Hk * 2 * kWaRows * D;
+    wa_bwd_setup(a, dtype);
+    return (unsigned long long)B * Hq * Tq + (unsigned long long)a.sink_tiles * a.splits * B * Hk * 2 * a.keys * D;
 }
 
 GFPP_API int gfpp_window_attn_backward(const void *q, const void *k, const void *v, const void *out, const void *out_low, const void *dout, const float *lse, void *dq, void *dk, void *dv,
@@ -364,11 +427,11 @@ GFPP_API int gfpp_window_attn_backward(const void *q, const void *k, const void 
     a.dv.p = dv;
     a.low = wa_two_part(Tk, left, right, sinks, dtype) ? const_cast<void *>(out_low) : nullptr;
     a.lse = const_cast<float *>(lse);
-    wa_bwd_setup(a);
+    wa_bwd_setup(a, dtype);
     a.delta = scratch;
     a.partial = scratch ? scratch + (uint64_t)B * Hq * Tq : nullptr;
     const uint64_t bh = (uint64_t)B * Hk, gq = (uint64_t)div_up(Tq, kWaRows) * Hq * B;
-    const uint64_t gk = ((uint64_t)div_up(Tk, kWaRows) - a.sink_tiles + (uint64_t)a.sink_tiles * a.splits) * bh;
+    const uint64_t gk = ((uint64_t)div_up(Tk, (uint32_t)a.keys) - a.sink_tiles + (uint64_t)a.sink_tiles * a.splits) * bh;
     WA_REQUIRE(gq <= 0x7fffffffull && gk <= 0x7fffffffull && (a.sink_tiles == 0 || (bh <= 65535 && a.sink_tiles <= 65535)));
     const size_t size = dtype == GFPP_F32 ? 4 : 2;
     bool vec = (uintptr_t)a.low % 16 == 0;

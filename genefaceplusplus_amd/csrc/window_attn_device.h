@@ -14,7 +14,7 @@
 
 namespace gfpp {
 
-constexpr int kWaThreads = 256, kWaRows = 128;      // four wavefronts of 32 queries (forward, dq) or 32 keys (dk, dv)
+constexpr int kWaThreads = 256, kWaRows = 128;      // four wavefronts of 32 queries (forward, dq); dk and dv: 128 keys, eight wavefronts
 
 template <bool B>
 struct WaFlag {
@@ -28,14 +28,25 @@ struct WaArgs {
     WaTensor q, k, v, o, dout, dq, dk, dv;
     void *low;                     // out's rounding errors (o's strides), or NULL
     float *lse, *delta;            // [B][Hq][Tq]
-    float *partial;                // sink tiles' dk and dv: [sink tiles][splits][B][Hk][2][128][D]
+    float *partial;                // sink tiles' dk and dv: [sink tiles][splits][B][Hk][2][keys][D]
     const int32_t *lengths;        // [B] or NULL
     int32_t B, Tq, Tk, Hq, Hk, D, G;
     int32_t left, right, sinks;    // left, right < 2^30
     int32_t q_start;
     float scale, c;                // c = scale log2(e)
     uint32_t sink_tiles, splits;
+    int32_t keys;                  // of a workgroup of dk and dv
 };
+
+// two query heads per workgroup: an even group, and enough workgroups left to fill the chip (a workgroup of either kind has its CU's registers to itself in pairs)
+inline bool wa_pair_heads(const WaArgs &a, uint64_t grid) { return a.G % 2 == 0 && grid / 2 >= (uint64_t)cu_count(); }
+
+// Workgroups are dealt out to the 8 XCDs in turn, each with an L2 of its own: the work items of one XCD are made neighbours (which read the same keys or
+// queries) by giving it a contiguous stretch of them.  A permutation of 0 .. total - 1 for any total.
+__device__ __forceinline__ uint32_t wa_item(uint32_t block, uint32_t total) {
+    const uint32_t xcd = block % 8, each = total / 8, more = total % 8;
+    return xcd * each + (xcd < more ? xcd : more) + block / 8;
+}
 
 template <typename T>
 struct WaTraits;
@@ -65,39 +76,47 @@ constexpr int wa_pitch_col() { return DP * (int)sizeof(T) % 128 == 0 ? DP * (int
 template <typename T, int DP>
 constexpr int wa_pitch_both() { return DP * (int)sizeof(T) + (sizeof(T) == 2 ? (DP == 32 ? 16 : 80) : 16); }
 
-// rows r0 .. r0 + ROWS - 1 of a [tokens][D] head into registers, the thread's share: 16 bytes per vector.  Rows from `end` on and columns from D on are zeros and
-// are not read: what lies behind a sequence may hold anything.
-template <typename T, int DP, int ROWS, bool VEC>
+// Rows r0 .. r0 + ROWS - 1 of a [tokens][D] head into registers, the thread's share: 16 bytes per vector.  Rows from `end` on and columns from D on are zeros and
+// are not read: what lies behind a sequence may hold anything.  VEC: buffer loads, whose range check gives those zeros without a branch or a clear per vector -- the
+// tile's base and its end are scalar, a lane keeps ONE 32-bit offset for all its vectors (the host has seen to it that 64 rows span less than 2^31 bytes and
+// that a row's pitch is at least its width).
+template <typename T, int DP, int ROWS, bool VEC, int THREADS = kWaThreads>
 struct WaStage {
-    static constexpr int V = WaTraits<T>::V, PER_ROW = DP / V, N = ROWS * PER_ROW / kWaThreads;
-    static_assert(ROWS * PER_ROW % kWaThreads == 0, "whole vectors per thread");
+    static constexpr int V = WaTraits<T>::V, PER_ROW = DP / V, ALL = ROWS * PER_ROW, N = (ALL + THREADS - 1) / THREADS, STEP = THREADS / PER_ROW;      // rows between a lane's vectors
+    static_assert(ALL % THREADS == 0 || ALL < THREADS, "whole vectors per thread, or one for some of them");
     typedef T vec __attribute__((ext_vector_type(V)));
     vec r[N];
 
+    // r0 >= 0 and the same in all lanes
     __device__ __forceinline__ void load(const T *base, int64_t stride, int r0, int end, int D) {
+        const T *tile = base + (int64_t)r0 * stride;
+        const int row = (int)threadIdx.x / PER_ROW, col = (int)threadIdx.x % PER_ROW * V;
+        if constexpr (VEC) {
+            const int rows = end - r0 < ROWS ? (end - r0 > 0 ? end - r0 : 0) : ROWS, pitch = (int)stride * (int)sizeof(T);
+            const auto rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<T *>(tile), 0, rows * pitch, 0x00020000);
+            const uint32_t at = col < D && (ALL >= THREADS || (int)threadIdx.x < ALL) ? (uint32_t)(row * pitch + col * (int)sizeof(T)) : 0x7ffffff0u;
 #pragma unroll
-        for (int n = 0; n < N; ++n) {
-            const int i = n * kWaThreads + (int)threadIdx.x, row = r0 + i / PER_ROW, col = i % PER_ROW * V;
-            vec t = (vec)(T)0.0f;
-            if (row < end && row >= 0 && col < D) {
-                const T *p = base + (int64_t)row * stride + col;
-                if constexpr (VEC) {
-                    t = *reinterpret_cast<const vec *>(p);
-                } else {
+            for (int n = 0; n < N; ++n)                        // (the whole offset in the lane: the range check subtracts a scalar offset from the size, without a sign)
+                r[n] = __builtin_bit_cast(vec, __builtin_amdgcn_raw_buffer_load_b128(rsrc, (int)(at + (uint32_t)(n * STEP * pitch)), 0, 0));
+        } else {
+#pragma unroll
+            for (int n = 0; n < N; ++n) {
+                vec t = (vec)(T)0.0f;
+                if (row + n * STEP < end - r0 && (ALL >= THREADS || (int)threadIdx.x < ALL)) {
+                    const T *p = tile + (int64_t)(row + n * STEP) * stride + col;
 #pragma unroll
                     for (int e = 0; e < V; ++e)
                         if (col + e < D) t[e] = p[e];
                 }
+                r[n] = t;
             }
-            r[n] = t;
         }
     }
     __device__ __forceinline__ void store(unsigned char *lds, int pitch) const {
+        unsigned char *at = lds + (int)threadIdx.x / PER_ROW * pitch + (int)threadIdx.x % PER_ROW * 16;
+        if (ALL >= THREADS || (int)threadIdx.x < ALL)
 #pragma unroll
-        for (int n = 0; n < N; ++n) {
-            const int i = n * kWaThreads + (int)threadIdx.x;
-            *reinterpret_cast<vec *>(lds + i / PER_ROW * pitch + i % PER_ROW * 16) = r[n];
-        }
+            for (int n = 0; n < N; ++n) *reinterpret_cast<vec *>(at + n * STEP * pitch) = r[n];
     }
 };
 
@@ -182,6 +201,31 @@ __device__ __forceinline__ void wa_arrived(V (&f)[N]) {
         }
     }
 }
+
+// N matrix instructions whose LDS operands are read kWaAhead instructions before their use.  Left to itself the compiler reads two fragments, waits for them and
+// multiplies: an LDS latency per two instructions, with which 35 % of the matrix pipe's cycles were used.  `read(x)`: fragment of instruction x, `use(x, f)`: the
+// instruction.  The barriers pin the order; prime() is called where the reads may start (in front of the arithmetic that the first instruction waits for).
+template <typename T, int N>
+struct WaStream {
+    typedef typename LpTraits<T>::vec vec;
+    static constexpr int AHEAD = (sizeof(T) == 4 ? 2 : 4) < N ? (sizeof(T) == 4 ? 2 : 4) : N;
+    vec ring[AHEAD];
+    template <typename Read>
+    __device__ __forceinline__ void prime(Read read) {
+#pragma unroll
+        for (int x = 0; x < AHEAD; ++x) ring[x] = read(x);
+        __builtin_amdgcn_sched_barrier(0);
+    }
+    template <typename Read, typename Use>
+    __device__ __forceinline__ void run(Read read, Use use) {
+#pragma unroll
+        for (int x = 0; x < N; ++x) {
+            use(x, ring[x % AHEAD]);
+            if (x + AHEAD < N) ring[x % AHEAD] = read(x + AHEAD);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    }
+};
 
 // values 8 s .. 8 s + 7 of a product, rounded to the operand type (pairs: one conversion instruction each)
 template <typename T>

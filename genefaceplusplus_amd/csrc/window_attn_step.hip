@@ -8,6 +8,7 @@
 // layout): keys come straight from memory as row fragments, values pass through a wavefront's own 32 rows of LDS for the transposing read.  A wavefront takes every
 // fourth tile of 32 slots of its workgroup's stretch, the next tile in flight in registers; the four partial softmaxes meet in LDS.  Few streams: the
 // slots of a stream are split over several workgroups, whose partial results a second launch joins.
+// Probabilities enter the products as a rounded value and its rounded remainder, so that the output carries its own rounding alone.
 // The row of the new token is taken from the arguments by whoever reads that slot, and written by one wavefront: no order between workgroups is needed.
 #include "window_attn_device.h"
 
@@ -133,6 +134,13 @@ __global__ __launch_bounds__(kWaThreads, sizeof(T) == 2 ? 2 : 1) void k_window_a
             const vec pr = wa_pack<T>(s, x);
 #pragma unroll
             for (int t = 0; t < NT; ++t) acc[t] = LpTraits<T>::mfma(wa_col<T, PV>(mine + col_at, 16 * x, t), pr, acc[t]);
+            if constexpr (sizeof(T) == 2) {                    // what the rounding left of them: the products are not what bounds this kernel
+#pragma unroll
+                for (int e = 0; e < 8; ++e) s[8 * x + e] -= (float)pr[e];
+                const vec rest = wa_pack<T>(s, x);
+#pragma unroll
+                for (int t = 0; t < NT; ++t) acc[t] = LpTraits<T>::mfma(wa_col<T, PV>(mine + col_at, 16 * x, t), rest, acc[t]);
+            }
         }
     }
     l = half_wave_sum(l);
@@ -200,11 +208,12 @@ static void ws_launch(const WsArgs &a, bool vec, uint32_t grid, hipStream_t st) 
     if (a.splits > 1) k_window_attn_step_join<T><<<(uint32_t)a.B * a.Hq, 128, 0, st>>>(a);
 }
 
-// stretches of a stream's slots: enough workgroups for four per CU, at least 256 slots (two tiles per wavefront) each
+// stretches of a stream's slots: enough workgroups for four per CU, at least 512 slots (four tiles per wavefront) each: below, the second launch costs what the
+// stretches save
 static uint32_t ws_splits(uint32_t B, uint32_t Hq, uint32_t Hk, uint32_t slots) {
     const uint64_t groups = (uint64_t)B * Hk * (((uint64_t)Hq / Hk + 31) / 32);
     if (groups == 0) return 1;
-    const uint64_t want = ((uint64_t)cu_count() * 4 + groups - 1) / groups, most = (slots + 255) / 256;
+    const uint64_t want = ((uint64_t)cu_count() * 4 + groups - 1) / groups, most = slots / 512;
     const uint64_t n = want < most ? want : most;
     return n < 1 ? 1 : (uint32_t)n;
 }

@@ -25,7 +25,7 @@ _lib.register("gfpp_rotary", [_p, _strides, _u32, _p] * 2 + [_p, _i, _i64, _p, c
 _lib.register("gfpp_window_attn_two_part", [_u32] + [_i32] * 3 + [_i])
 _lib.register("gfpp_window_attn_forward", [_p] * 6 + [_strides] + [_u32] * 6 + [_i32] * 4 + [_p, _f, _i, _p])
 _lib.register("gfpp_window_attn_backward", [_p] * 11 + [_strides] + [_u32] * 6 + [_i32] * 4 + [_p, _f, _i, _p])
-_lib.register("gfpp_window_attn_backward_scratch_floats", [_u32] * 6 + [_i32] * 3, restype=ctypes.c_uint64)
+_lib.register("gfpp_window_attn_backward_scratch_floats", [_u32] * 6 + [_i32] * 4 + [_i], restype=ctypes.c_uint64)
 _lib.register("gfpp_window_attn_step", [_p] * 6 + [_i, _p, _strides] + [_u32] * 6 + [_f, _i, _p, _p])
 _lib.register("gfpp_window_attn_step_scratch_floats", [_u32] * 5, restype=ctypes.c_uint64)
 _SYMBOLS = ("gfpp_last_error", "gfpp_layer_norm_forward", "gfpp_layer_norm_backward", "gfpp_layer_norm_backward_scratch_floats", "gfpp_rotary", "gfpp_window_attn_two_part",

@@ -888,7 +888,7 @@ int gfpp_window_attn_backward(const void *q, const void *k, const void *v, const
                               int32_t right, int32_t sinks, int32_t q_start, const int32_t *lengths, float scale, int dtype, gfpp_stream_t stream);
 /* (cond_encoder.py:146-180, as above) */
 unsigned long long gfpp_window_attn_backward_scratch_floats(uint32_t B, uint32_t Tq, uint32_t Tk, uint32_t Hq, uint32_t Hk, uint32_t D, int32_t left,
-                                                            int32_t sinks, int32_t q_start);
+                                                            int32_t right, int32_t sinks, int32_t q_start, int dtype);
 
 /* One new token per stream (AudioAttNet's weighted window, cond_encoder.py:146-180, for a live stream): stream b's token at positions[b] (int32, or int64 with
  * positions64) writes k[b], v[b] [Hk, D] into its slot of cache_k, cache_v [B, slots, Hk, D] -- n < sinks ? n : sinks + (n - sinks) mod (slots - sinks) -- and

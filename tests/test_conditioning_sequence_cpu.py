@@ -155,8 +155,8 @@ def test_c_entry_refusals():
     for bad in (dict(dt=9), dict(Hq=3, Hk=2), dict(left=-1), dict(scale=nan), dict(start=-5)):
         assert attn_bwd(**bad) == EINVAL, bad
     assert attn_bwd(D=200) == EUNSUPPORTED and attn_bwd(B=0) == 0
-    assert lib.gfpp_window_attn_backward_scratch_floats(2, 100, 100, 4, 2, 64, 10, 3, 0) == 2 * 4 * 100        # short: the sinks' tile is one workgroup's
-    assert lib.gfpp_window_attn_backward_scratch_floats(1, 4096, 4096, 4, 2, 64, 10, 3, 0) > 4 * 4096         # long: slices
+    assert lib.gfpp_window_attn_backward_scratch_floats(2, 100, 100, 4, 2, 64, 10, 0, 3, 0, 0) == 2 * 4 * 100        # short: the sinks' tile is one workgroup's
+    assert lib.gfpp_window_attn_backward_scratch_floats(1, 4096, 4096, 4, 2, 64, 10, 0, 3, 0, 0) > 4 * 4096         # long: slices
 
     def step(q=P, k=P, v=P, ck=P, cv=P, pos=P, o=P, st=s(14), B=1, Hq=2, Hk=1, D=8, slots=100, sinks=2, scale=1.0, dt=0, scratch=None):
         return lib.gfpp_window_attn_step(q, k, v, ck, cv, pos, 0, o, st, B, Hq, Hk, D, slots, sinks, scale, dt, scratch, None)
