@@ -12,31 +12,35 @@
 
 namespace gfpp {
 
-template <typename T, int DP>
-constexpr int wa_bn() { return sizeof(T) == 4 && DP == 128 ? 32 : 64; }
+// Keys per tile.  64 let one half's products run under the other's arithmetic where registers allow it (128-wide 16-bit heads); up to 64 features 32 keys fit four wavefronts to a
+// SIMD instead of three (13 000 x 8 heads x 64, window 1024: 78 -> 71 us), and a query that sees few keys has less of a tile to mask.
+template <typename T, int DP, bool FEW>
+constexpr int wa_bn() { return FEW || (sizeof(T) == 4 && DP == 128) || (sizeof(T) == 2 && DP <= 64) ? 32 : 64; }
 
-// TWO: probabilities as a rounded value and its remainder (window_attn_device.h: wa_two_part).  HEADS 2: eight wavefronts, four for each of two query heads of a
-// group, share the tiles of keys and values -- half the loads and LDS writes per query.
-template <typename T, int DP, bool VEC, bool TWO, int HEADS>
-__global__ __launch_bounds__(kWaThreads * HEADS, sizeof(T) == 2 ? (DP <= 64 && VEC ? 3 : (VEC || HEADS == 2 ? 2 : 1)) : 1) void k_window_attn(WaArgs a) {
-    constexpr int BN = wa_bn<T, DP>(), NS = DP / 16, NT = DP / 32, NSUB = BN / 32, PK = wa_pitch_row<T, DP>(), PV = wa_pitch_col<T, DP>();
+// FEW: a query sees at most 64 keys (wa_few): small tiles, and in the 16-bit modes probabilities as a rounded value and its remainder (window_attn_device.h).
+// HEADS 2: eight wavefronts, four for each of two query heads of a group, share the tiles of keys and values -- half the loads and LDS writes per query.
+// WAVES 1: 32 queries a workgroup instead of 128, for few keys and a grid that would leave CUs empty.
+template <typename T, int DP, bool VEC, bool FEW, int HEADS, int WAVES>
+__global__ __launch_bounds__(64 * WAVES * HEADS, WAVES == 1 ? 1 : (sizeof(T) == 2 ? (DP <= 64 && VEC ? (FEW ? 3 : 4) : (VEC || HEADS == 2 ? 2 : 1)) : 1)) void k_window_attn(WaArgs a) {
+    constexpr int BN = wa_bn<T, DP, FEW>(), ROWS = 32 * WAVES, NS = DP / 16, NT = DP / 32, NSUB = BN / 32, PK = wa_pitch_row<T, DP>(), PV = wa_pitch_col<T, DP>();
+    constexpr bool TWO = FEW && sizeof(T) == 2;
     typedef typename LpTraits<T>::vec vec;
     __shared__ __attribute__((aligned(16))) unsigned char s_k[2][BN * PK], s_v[2][BN * PV];
-    const int q_tiles = (a.Tq + kWaRows - 1) / kWaRows;
+    const int q_tiles = (a.Tq + ROWS - 1) / ROWS;
     // items: sequence, key head, tile of queries, query head of the group -- those that read the same keys side by side
     uint32_t item = wa_item(blockIdx.x, gridDim.x);
-    const int in_group = (int)(item % (a.G / HEADS)) * HEADS + (HEADS == 2 ? __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 8)) : 0);
+    const int in_group = (int)(item % (a.G / HEADS)) * HEADS + (HEADS == 2 ? __builtin_amdgcn_readfirstlane((int)(threadIdx.x / (64 * WAVES))) : 0);
     item /= a.G / HEADS;
-    const int i0 = (int)(item % q_tiles) * kWaRows;
+    const int i0 = (int)(item % q_tiles) * ROWS;
     item /= q_tiles;
     const int hk = (int)(item % a.Hk), hq = hk * a.G + in_group, b = (int)(item / a.Hk);
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6) & 3), c = lane & 31, h = lane >> 5;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6) % WAVES), c = lane & 31, h = lane >> 5;
     const int n = a.lengths ? a.lengths[b] < a.Tk ? a.lengths[b] : a.Tk : a.Tk;
     const int i = i0 + wave * 32 + c, p = a.q_start + i;
     const bool have = i < a.Tq && p < n;
     vec q[NS];
     wa_global_rows<T, NS, VEC>(q, static_cast<const T *>(a.q.p) + b * a.q.sb + (int64_t)i * a.q.st + hq * a.q.sh, have, h, a.D);
-    const int i1 = i0 + kWaRows < a.Tq ? i0 + kWaRows - 1 : a.Tq - 1;
+    const int i1 = i0 + ROWS < a.Tq ? i0 + ROWS - 1 : a.Tq - 1;
     const WaRange range = wa_keys<BN>(a, a.q_start + i0, a.q_start + i1, n);
     const int tiles = range.head + range.hi - range.lo;
     const int last = have ? (p + a.right < n - 1 ? p + a.right : n - 1) : -1, first = p - a.left;          // this lane's query
@@ -48,29 +52,35 @@ __global__ __launch_bounds__(kWaThreads * HEADS, sizeof(T) == 2 ? (DP <= 64 && V
         for (int r = 0; r < 16; ++r) acc[t][r] = 0.0f;
     float m = -INFINITY, l = 0.0f;
     const T *kb = static_cast<const T *>(a.k.p) + b * a.k.sb + hk * a.k.sh, *vb = static_cast<const T *>(a.v.p) + b * a.v.sb + hk * a.v.sh;
-    WaStage<T, DP, BN, VEC, kWaThreads * HEADS> rk, rv;
+    // two tiles in flight: the one that the next step stores and the one after it (one alone arrives later than the step that it was requested in takes)
+    WaStage<T, DP, BN, VEC, 64 * WAVES * HEADS> rk[2], rv[2];
     auto tile_row = [&](int k) { return (k < range.head ? k : range.lo + k - range.head) * BN; };
     if (tiles > 0) {
-        rk.load(kb, a.k.st, tile_row(0), n, a.D);
-        rv.load(vb, a.v.st, tile_row(0), n, a.D);
-        rk.store(s_k[0], PK);
-        rv.store(s_v[0], PV);
+        rk[0].load(kb, a.k.st, tile_row(0), n, a.D);
+        rv[0].load(vb, a.v.st, tile_row(0), n, a.D);
         if (tiles > 1) {
-            rk.load(kb, a.k.st, tile_row(1), n, a.D);
-            rv.load(vb, a.v.st, tile_row(1), n, a.D);
+            rk[1].load(kb, a.k.st, tile_row(1), n, a.D);
+            rv[1].load(vb, a.v.st, tile_row(1), n, a.D);
+        }
+        rk[0].store(s_k[0], PK);
+        rv[0].store(s_v[0], PV);
+        if (tiles > 2) {
+            rk[0].load(kb, a.k.st, tile_row(2), n, a.D);
+            rv[0].load(vb, a.v.st, tile_row(2), n, a.D);
         }
     }
     wa_arrived(q);
     __syncthreads();
     const int row_at = c * PK + 8 * h * (int)sizeof(T), col_at = wa_col_offset<T>(lane, PV);
-    for (int k = 0; k < tiles; ++k) {
-        const int buf = k & 1, j0 = tile_row(k), j1 = j0 + BN - 1;
+    auto step = [&](int k, auto which) {
+        constexpr int buf = decltype(which)::value, other = buf ^ 1;     // of tile k (LDS) and of tile k + 1 (LDS, registers)
+        const int j0 = tile_row(k), j1 = j0 + BN - 1;
         if (k + 1 < tiles) {
-            rk.store(s_k[buf ^ 1], PK);                     // (last read before the previous barrier)
-            rv.store(s_v[buf ^ 1], PV);
-            if (k + 2 < tiles) {
-                rk.load(kb, a.k.st, tile_row(k + 2), n, a.D);
-                rv.load(vb, a.v.st, tile_row(k + 2), n, a.D);
+            rk[other].store(s_k[other], PK);                     // (last read before the previous barrier)
+            rv[other].store(s_v[other], PV);
+            if (k + 3 < tiles) {
+                rk[other].load(kb, a.k.st, tile_row(k + 3), n, a.D);
+                rv[other].load(vb, a.v.st, tile_row(k + 3), n, a.D);
             }
         }
         const bool seen = pw0 < n && j0 <= pw1 + a.right && (j1 >= pw0 - a.left || j0 < a.sinks);
@@ -147,6 +157,10 @@ __global__ __launch_bounds__(kWaThreads * HEADS, sizeof(T) == 2 ? (DP <= 64 && V
             }
         }
         __syncthreads();
+    };
+    for (int k = 0; k < tiles; k += 2) {
+        step(k, WaInt<0>{});
+        if (k + 1 < tiles) step(k + 1, WaInt<1>{});
     }
     l = half_wave_sum(l);
     if (i >= a.Tq) return;
@@ -207,19 +221,25 @@ int wa_arguments(const char *what, WaArgs &a, const int64_t *strides, int n_tens
     return 0;
 }
 
-template <typename T, int DP, bool TWO, int HEADS>
-static void wa_forward_launch(const WaArgs &a, bool vec, uint32_t grid, hipStream_t st) {
-    if (vec) k_window_attn<T, DP, true, TWO, HEADS><<<grid / HEADS, kWaThreads * HEADS, 0, st>>>(a);
-    else k_window_attn<T, DP, false, TWO, HEADS><<<grid / HEADS, kWaThreads * HEADS, 0, st>>>(a);
+template <typename T, int DP, bool FEW, int HEADS, int WAVES>
+static void wa_forward_launch(const WaArgs &a, bool vec, hipStream_t st) {
+    const uint32_t grid = div_up((uint32_t)a.Tq, 32 * WAVES) * (uint32_t)(a.Hq / HEADS) * (uint32_t)a.B;
+    if (vec) k_window_attn<T, DP, true, FEW, HEADS, WAVES><<<grid, 64 * WAVES * HEADS, 0, st>>>(a);
+    else if constexpr (HEADS == 1) k_window_attn<T, DP, false, FEW, HEADS, WAVES><<<grid, 64 * WAVES, 0, st>>>(a);
 }
-template <typename T, bool TWO>
-static void wa_forward(const WaArgs &a, bool vec, uint32_t grid, hipStream_t st) {
-    if (a.D <= 32) wa_forward_launch<T, 32, TWO, 1>(a, vec, grid, st);
-    else if (a.D <= 64) wa_forward_launch<T, 64, TWO, 1>(a, vec, grid, st);
-    else if constexpr (sizeof(T) == 2 && !TWO) {
-        if (vec && wa_pair_heads(a, grid)) k_window_attn<T, 128, true, TWO, 2><<<grid / 2, kWaThreads * 2, 0, st>>>(a);
-        else wa_forward_launch<T, 128, TWO, 1>(a, vec, grid, st);
-    } else wa_forward_launch<T, 128, TWO, 1>(a, vec, grid, st);
+template <typename T, int DP>
+static void wa_forward_width(const WaArgs &a, bool vec, bool few, uint32_t grid, hipStream_t st) {
+    if constexpr (DP * sizeof(T) <= 128)                       // (wider rows: a wavefront alone has no registers for two tiles in flight)
+        if (few && grid < 2u * (uint32_t)cu_count()) return wa_forward_launch<T, DP, true, 1, 1>(a, vec, st);
+    if constexpr (DP == 128 && sizeof(T) == 2)
+        if (!few && vec && wa_pair_heads(a, grid)) return wa_forward_launch<T, DP, false, 2, 4>(a, vec, st);
+    few ? wa_forward_launch<T, DP, true, 1, 4>(a, vec, st) : wa_forward_launch<T, DP, false, 1, 4>(a, vec, st);
+}
+template <typename T>
+static void wa_forward(const WaArgs &a, bool vec, bool few, uint32_t grid, hipStream_t st) {
+    if (a.D <= 32) wa_forward_width<T, 32>(a, vec, few, grid, st);
+    else if (a.D <= 64) wa_forward_width<T, 64>(a, vec, few, grid, st);
+    else wa_forward_width<T, 128>(a, vec, few, grid, st);
 }
 
 }  // namespace gfpp
@@ -241,15 +261,15 @@ GFPP_API int gfpp_window_attn_forward(const void *q, const void *k, const void *
     a.v.p = const_cast<void *>(v);
     a.o.p = out;
     a.lse = lse;
-    const bool two = wa_two_part(Tk, left, right, sinks, dtype);
-    a.low = two ? out_low : nullptr;
+    const bool few = wa_few(Tk, left, right, sinks);
+    a.low = wa_two_part(Tk, left, right, sinks, dtype) ? out_low : nullptr;
     const uint64_t grid = (uint64_t)div_up(Tq, kWaRows) * Hq * B;
     WA_REQUIRE(grid <= 0x7fffffffull);
     const size_t size = dtype == GFPP_F32 ? 4 : 2;
     const bool vec = wa_vectors(a.q, a.D, size) && wa_vectors(a.k, a.D, size) && wa_vectors(a.v, a.D, size) && wa_vectors(a.o, a.D, size) && (uintptr_t)a.low % 16 == 0;
     hipStream_t st = (hipStream_t)stream;
-    if (dtype == GFPP_F32) wa_forward<float, false>(a, vec, (uint32_t)grid, st);
-    else if (dtype == GFPP_F16) two ? wa_forward<_Float16, true>(a, vec, (uint32_t)grid, st) : wa_forward<_Float16, false>(a, vec, (uint32_t)grid, st);
-    else two ? wa_forward<__bf16, true>(a, vec, (uint32_t)grid, st) : wa_forward<__bf16, false>(a, vec, (uint32_t)grid, st);
+    if (dtype == GFPP_F32) wa_forward<float>(a, vec, few, (uint32_t)grid, st);
+    else if (dtype == GFPP_F16) wa_forward<_Float16>(a, vec, few, (uint32_t)grid, st);
+    else wa_forward<__bf16>(a, vec, few, (uint32_t)grid, st);
     return check_launch(what);
 }

@@ -19,7 +19,7 @@ bool wa_vectors(const WaTensor &t, int D, size_t size);
 // (HEADS: as in the forward pass)
 template <typename T, int DP, bool VEC, int HEADS>
 __global__ __launch_bounds__(kWaThreads * HEADS, sizeof(T) == 2 && (VEC || DP <= 64) ? 2 : 1) void k_window_attn_dq(WaArgs a) {
-    constexpr int BN = sizeof(T) == 4 && DP == 128 ? 32 : 64, NS = DP / 16, NT = DP / 32, PK = wa_pitch_both<T, DP>(), PV = wa_pitch_row<T, DP>();
+    constexpr int BN = DP == 128 && (sizeof(T) == 4 || HEADS == 1) ? 32 : 64, NS = DP / 16, NT = DP / 32, PK = wa_pitch_both<T, DP>(), PV = wa_pitch_row<T, DP>();
     typedef typename LpTraits<T>::vec vec;
     __shared__ __attribute__((aligned(16))) unsigned char s_k[2][BN * PK], s_v[2][BN * PV];
     const int q_tiles = (a.Tq + kWaRows - 1) / kWaRows;
@@ -71,30 +71,36 @@ __global__ __launch_bounds__(kWaThreads * HEADS, sizeof(T) == 2 && (VEC || DP <=
 #pragma unroll
         for (int r = 0; r < 16; ++r) acc[t][r] = 0.0f;
     const T *kb = static_cast<const T *>(a.k.p) + b * a.k.sb + hk * a.k.sh, *vb = static_cast<const T *>(a.v.p) + b * a.v.sb + hk * a.v.sh;
-    WaStage<T, DP, BN, VEC, kWaThreads * HEADS> rk, rv;
+    // two tiles in flight: the one that the next step stores and the one after it (one alone arrives later than the step that it was requested in takes)
+    WaStage<T, DP, BN, VEC, kWaThreads * HEADS> rk[2], rv[2];
     auto tile_row = [&](int k) { return (k < range.head ? k : range.lo + k - range.head) * BN; };
     if (tiles > 0) {
-        rk.load(kb, a.k.st, tile_row(0), n, a.D);
-        rv.load(vb, a.v.st, tile_row(0), n, a.D);
-        rk.store(s_k[0], PK);
-        rv.store(s_v[0], PV);
+        rk[0].load(kb, a.k.st, tile_row(0), n, a.D);
+        rv[0].load(vb, a.v.st, tile_row(0), n, a.D);
         if (tiles > 1) {
-            rk.load(kb, a.k.st, tile_row(1), n, a.D);
-            rv.load(vb, a.v.st, tile_row(1), n, a.D);
+            rk[1].load(kb, a.k.st, tile_row(1), n, a.D);
+            rv[1].load(vb, a.v.st, tile_row(1), n, a.D);
+        }
+        rk[0].store(s_k[0], PK);
+        rv[0].store(s_v[0], PV);
+        if (tiles > 2) {
+            rk[0].load(kb, a.k.st, tile_row(2), n, a.D);
+            rv[0].load(vb, a.v.st, tile_row(2), n, a.D);
         }
     }
     wa_arrived(q);
     wa_arrived(g);
     __syncthreads();
     const int row_k = c * PK + 8 * h * (int)sizeof(T), row_v = c * PV + 8 * h * (int)sizeof(T), col_at = wa_col_offset<T>(lane, PK);
-    for (int k = 0; k < tiles; ++k) {
-        const int buf = k & 1, j0 = tile_row(k), j1 = j0 + BN - 1;
+    auto step = [&](int k, auto which) {
+        constexpr int buf = decltype(which)::value, other = buf ^ 1;
+        const int j0 = tile_row(k), j1 = j0 + BN - 1;
         if (k + 1 < tiles) {
-            rk.store(s_k[buf ^ 1], PK);
-            rv.store(s_v[buf ^ 1], PV);
-            if (k + 2 < tiles) {
-                rk.load(kb, a.k.st, tile_row(k + 2), n, a.D);
-                rv.load(vb, a.v.st, tile_row(k + 2), n, a.D);
+            rk[other].store(s_k[other], PK);
+            rv[other].store(s_v[other], PV);
+            if (k + 3 < tiles) {
+                rk[other].load(kb, a.k.st, tile_row(k + 3), n, a.D);
+                rv[other].load(vb, a.v.st, tile_row(k + 3), n, a.D);
             }
         }
         const bool seen = pw0 < n && j0 <= pw1 + a.right && (j1 >= pw0 - a.left || j0 < a.sinks);
@@ -134,6 +140,10 @@ __global__ __launch_bounds__(kWaThreads * HEADS, sizeof(T) == 2 && (VEC || DP <=
             }
         }
         __syncthreads();
+    };
+    for (int k = 0; k < tiles; k += 2) {
+        step(k, WaInt<0>{});
+        if (k + 1 < tiles) step(k + 1, WaInt<1>{});
     }
     if (i < a.Tq) wa_store_rows<T, NT, VEC>(acc, a.scale, static_cast<T *>(a.dq.p) + b * a.dq.sb + (int64_t)i * a.dq.st + hq * a.dq.sh, h, a.D);
 }
@@ -146,7 +156,7 @@ __global__ __launch_bounds__(kWaThreads * HEADS, sizeof(T) == 2 && (VEC || DP <=
 // PAIRS: of wavefronts, 32 keys each: 4, or 2 where 128 keys a workgroup would leave CUs without one (and for the widest fp32 heads, which need the registers).
 constexpr int kWaBq = 32;
 template <typename T, int DP, bool VEC, int PAIRS>
-__global__ __launch_bounds__(PAIRS * 128, sizeof(T) == 4 && DP == 128 ? 1 : 2) void k_window_attn_dkv(WaArgs a) {
+__global__ __launch_bounds__(PAIRS * 128, PAIRS == 2 && DP == 128 && (sizeof(T) == 4 || !VEC) ? 1 : 2) void k_window_attn_dkv(WaArgs a) {
     constexpr int KEYS = PAIRS * 32, BQ = kWaBq, NS = DP / 16, NT = DP / 32, PITCH = wa_pitch_both<T, DP>();
     typedef typename LpTraits<T>::vec vec;
     typedef float f4 __attribute__((ext_vector_type(4)));
@@ -189,45 +199,47 @@ __global__ __launch_bounds__(PAIRS * 128, sizeof(T) == 4 && DP == 128 ? 1 : 2) v
         tiles = tiles < 0 ? 0 : tiles;
     }
     const int steps = tiles * a.G;
-    WaStage<T, DP, BQ, VEC, PAIRS * 128> rq, rg;
-    float r_stat = 0.0f;
+    WaStage<T, DP, BQ, VEC, PAIRS * 128> rq[2], rg[2];                                 // two tiles in flight (k_window_attn)
+    float r_stat[2] = {0.0f, 0.0f};
     int next_tile = 0, next_head = 0;                                                  // of the tile that is loaded next: the heads of a group one after the other
-    auto load = [&]() {
+    auto load = [&](int which) {
         const int hq = hk * a.G + next_head, i = i_lo + next_tile * BQ;
-        rq.load(static_cast<const T *>(a.q.p) + b * a.q.sb + hq * a.q.sh, a.q.st, i, end, a.D);
-        rg.load(static_cast<const T *>(a.dout.p) + b * a.dout.sb + hq * a.dout.sh, a.dout.st, i, end, a.D);
+        rq[which].load(static_cast<const T *>(a.q.p) + b * a.q.sb + hq * a.q.sh, a.q.st, i, end, a.D);
+        rg[which].load(static_cast<const T *>(a.dout.p) + b * a.dout.sb + hq * a.dout.sh, a.dout.st, i, end, a.D);
         if (threadIdx.x < 2 * BQ) {
             const int row = i + (int)(threadIdx.x % BQ);
             const int64_t at = ((int64_t)b * a.Hq + hq) * a.Tq + row;
-            if (threadIdx.x < BQ) r_stat = row < end ? a.lse[at] : INFINITY;
-            else r_stat = row < end ? a.delta[at] : 0.0f;
+            if (threadIdx.x < BQ) r_stat[which] = row < end ? a.lse[at] : INFINITY;
+            else r_stat[which] = row < end ? a.delta[at] : 0.0f;
         }
         if (++next_tile == tiles) {
             next_tile = 0;
             ++next_head;
         }
     };
-    auto store = [&](int buf) {
-        rq.store(s_q[buf], PITCH);
-        rg.store(s_g[buf], PITCH);
-        if (threadIdx.x < BQ) s_lse[buf][threadIdx.x] = r_stat;
-        else if (threadIdx.x < 2 * BQ) s_delta[buf][threadIdx.x - BQ] = r_stat;
+    auto store = [&](int buf, int which) {
+        rq[which].store(s_q[buf], PITCH);
+        rg[which].store(s_g[buf], PITCH);
+        if (threadIdx.x < BQ) s_lse[buf][threadIdx.x] = r_stat[which];
+        else if (threadIdx.x < 2 * BQ) s_delta[buf][threadIdx.x - BQ] = r_stat[which];
     };
     if (steps > 0) {
-        load();
-        store(0);
-        if (steps > 1) load();
+        load(0);
+        if (steps > 1) load(1);
+        store(0, 0);
+        if (steps > 2) load(0);
     }
     wa_arrived(f);
     __syncthreads();
     const int row_at = c * PITCH + 8 * h * (int)sizeof(T), col_at = wa_col_offset<T>(lane, PITCH);
     const int from = have ? j - a.right : 0x7fffffff, to = j < a.sinks ? 0x7fffffff : j + a.left;
     int now = 0, tile = second ? -1 : 0, buf = second ? 2 : 0;                         // buffer of step k; this wavefront's tile and its buffer (one step behind: second)
-    for (int k = 0; k <= steps; ++k) {
+    auto step = [&](int k, auto parity) {
+        constexpr int odd = decltype(parity)::value;                                   // k & 1; tile k + 1 is in the other registers
         const int next = now == 2 ? 0 : now + 1;
         if (k + 1 < steps) {
-            store(next);                                                               // (tile k - 2's: last read a step ago, before the barrier)
-            if (k + 2 < steps) load();
+            store(next, odd ^ 1);                                                      // (tile k - 2's: last read a step ago, before the barrier)
+            if (k + 3 < steps) load(odd ^ 1);
         }
         const int p0 = a.q_start + i_lo + tile * BQ, p1 = p0 + BQ - 1;
         const bool seen = jw0 < n && p1 >= jw0 - a.right && (p0 <= jw1 + a.left || jw0 < a.sinks);
@@ -258,7 +270,7 @@ __global__ __launch_bounds__(PAIRS * 128, sizeof(T) == 4 && DP == 128 ? 1 : 2) v
                     f4 pr;
 #pragma unroll
                     for (int e = 0; e < 4; ++e) pr[e] = s[r + e] = __builtin_amdgcn_exp2f(fmaf(s[r + e], a.c, -lse[e]));
-                    *reinterpret_cast<f4 *>(s_p[k & 1][keys][r >> 2][lane]) = pr;
+                    *reinterpret_cast<f4 *>(s_p[odd][keys][r >> 2][lane]) = pr;
                 }
                 vec pr;
                 cols.run(read_g, [&](int x, const vec &y) {
@@ -281,7 +293,7 @@ __global__ __launch_bounds__(PAIRS * 128, sizeof(T) == 4 && DP == 128 ? 1 : 2) v
             cols.prime(read_q);
 #pragma unroll
             for (int r = 0; r < 16; r += 4) {
-                const f4 delta = *reinterpret_cast<const f4 *>(&s_delta[buf][2 * r + 4 * h]), pr = *reinterpret_cast<const f4 *>(s_p[(k - 1) & 1][keys][r >> 2][lane]);
+                const f4 delta = *reinterpret_cast<const f4 *>(&s_delta[buf][2 * r + 4 * h]), pr = *reinterpret_cast<const f4 *>(s_p[odd ^ 1][keys][r >> 2][lane]);
 #pragma unroll
                 for (int e = 0; e < 4; ++e) d[r + e] = pr[e] * (d[r + e] - delta[e]);
             }
@@ -295,6 +307,10 @@ __global__ __launch_bounds__(PAIRS * 128, sizeof(T) == 4 && DP == 128 ? 1 : 2) v
         now = next;
         buf = buf == 2 ? 0 : buf + 1;
         if (++tile == tiles) tile = 0;
+    };
+    for (int k = 0; k <= steps; k += 2) {
+        step(k, WaInt<0>{});
+        if (k + 1 <= steps) step(k + 1, WaInt<1>{});
     }
     if (j >= a.Tk) return;
     const float f_out = second ? a.scale : 1.0f;

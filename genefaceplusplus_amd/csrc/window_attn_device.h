@@ -16,9 +16,9 @@ namespace gfpp {
 
 constexpr int kWaThreads = 256, kWaRows = 128;      // four wavefronts of 32 queries (forward, dq); dk and dv: 128 keys, eight wavefronts
 
-template <bool B>
-struct WaFlag {
-    static constexpr bool value = B;
+template <int N>
+struct WaInt {
+    static constexpr int value = N;
 };
 struct WaTensor {
     void *p;
@@ -309,10 +309,11 @@ __device__ __forceinline__ void wa_store_rows(const v16f (&acc)[NT], float f, T 
 // do not, and delta, the backward pass' row sum, carries both into every score gradient of the row.  Where a query sees at most 64 keys the forward pass therefore
 // takes its probabilities as a rounded value and a rounded remainder (a second product: such calls are bound by latency and memory), and a training pass keeps
 // the output's remainder for delta.  Goes by the arguments alone, so that a pass with gradients and one without give the same bits.
-__host__ __device__ inline bool wa_two_part(int64_t Tk, int64_t left, int64_t right, int64_t sinks, int dtype) {
+inline bool wa_few(int64_t Tk, int64_t left, int64_t right, int64_t sinks) {
     const int64_t window = left + right + 1 + sinks;
-    return dtype != GFPP_F32 && (window < Tk ? window : Tk) <= 64;
+    return (window < Tk ? window : Tk) <= 64;
 }
+inline bool wa_two_part(int64_t Tk, int64_t left, int64_t right, int64_t sinks, int dtype) { return dtype != GFPP_F32 && wa_few(Tk, left, right, sinks); }
 
 // tiles of BN keys that queries at positions p0 .. p1 can see: [0, head) for the sinks in front of the band, [lo, hi) for the band (merged where they touch)
 struct WaRange {
