@@ -63,10 +63,20 @@ __device__ __forceinline__ void ln_param(const void *p, bool f32, uint32_t at, f
     }
 }
 
+// sum over the wavefront, in a scalar register: data-parallel moves inside the vector unit (shifts within rows of 16 lanes, then row to row) instead of six round
+// trips through the LDS crossbar
+template <int CTRL, int ROWS>
+__device__ __forceinline__ float dpp_add(float v) {
+    return v + __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, ROWS, 0xf, false));
+}
 __device__ __forceinline__ float wave_sum(float v) {
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o);
-    return v;
+    v = dpp_add<0x111, 0xf>(v);                        // row_shr 1, 2, 4, 8: lane 15 of a row has its sum
+    v = dpp_add<0x112, 0xf>(v);
+    v = dpp_add<0x114, 0xf>(v);
+    v = dpp_add<0x118, 0xf>(v);
+    v = dpp_add<0x142, 0xa>(v);                        // row_bcast 15 into rows 1 and 3, row_bcast 31 into rows 2 and 3: lane 63 has all
+    v = dpp_add<0x143, 0xc>(v);
+    return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), 63));
 }
 // sum over the WG threads that share a row, in every one of them; `box`: LDS of one float per wavefront, free again after the next call's first barrier
 template <int TPR>
@@ -95,55 +105,62 @@ struct LnArgs {
     int param_f32;
 };
 
-// TPR threads per row (64: four rows per workgroup at a time, 256: one), NV vectors of VEC elements per thread
-template <typename T, int VEC, int TPR, int NV>
+// TPR threads per row (64: a wavefront, 256: the workgroup), NV vectors of VEC elements per thread, R rows of a wavefront at a time: their loads are in flight together
+template <typename T, int VEC, int TPR, int NV, int R>
 __global__ __launch_bounds__(256) void k_layer_norm(LnArgs a) {
     __shared__ float box[4];
     constexpr int RPW = 256 / TPR;
-    const uint32_t t = threadIdx.x % TPR, sub = threadIdx.x / TPR;
+    const uint32_t t = threadIdx.x % TPR, sub = TPR == 64 ? (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x / TPR)) : 0;
     const float n = (float)a.N;
-    for (uint64_t row0 = (uint64_t)blockIdx.x * RPW; row0 < a.M; row0 += (uint64_t)gridDim.x * RPW) {
-        const uint64_t row = row0 + sub;
-        if (TPR == 64 && row >= a.M) break;            // a whole wavefront: no barrier in this form
-        const T *x = static_cast<const T *>(a.x) + (int64_t)row * a.xs;
-        float v[NV][VEC];
-        float s = 0.0f;
+    for (uint64_t row0 = ((uint64_t)blockIdx.x * RPW + sub) * R; row0 < a.M; row0 += (uint64_t)gridDim.x * RPW * R) {      // (TPR 256: the same in all threads)
+        float v[R][NV][VEC];
 #pragma unroll
-        for (int k = 0; k < NV; ++k) {
-            const uint32_t c = (k * TPR + t) * VEC;
-            if (c < a.N) {
-                ln_load<T, VEC>(x + c, v[k]);
+        for (int q = 0; q < R; ++q) {
+            const T *x = static_cast<const T *>(a.x) + (int64_t)(row0 + q < a.M ? row0 + q : a.M - 1) * a.xs;            // (the last row again: nothing is written twice)
 #pragma unroll
-                for (int e = 0; e < VEC; ++e) s += v[k][e];
+            for (int k = 0; k < NV; ++k) {
+                const uint32_t c = (k * TPR + t) * VEC;
+                if (c < a.N) ln_load<T, VEC>(x + c, v[q][k]);
             }
         }
-        const float mean = row_sum<TPR>(s, box) / n;
-        s = 0.0f;
 #pragma unroll
-        for (int k = 0; k < NV; ++k)
-            if ((k * TPR + t) * VEC < a.N)
+        for (int q = 0; q < R; ++q) {
+            const uint64_t row = row0 + q;
+            if (row >= a.M) break;
+            float s = 0.0f;
 #pragma unroll
-                for (int e = 0; e < VEC; ++e) {
-                    const float d = v[k][e] - mean;
-                    s = fmaf(d, d, s);
+            for (int k = 0; k < NV; ++k)
+                if ((k * TPR + t) * VEC < a.N)
+#pragma unroll
+                    for (int e = 0; e < VEC; ++e) s += v[q][k][e];
+            const float mean = row_sum<TPR>(s, box) / n;
+            s = 0.0f;
+#pragma unroll
+            for (int k = 0; k < NV; ++k)
+                if ((k * TPR + t) * VEC < a.N)
+#pragma unroll
+                    for (int e = 0; e < VEC; ++e) {
+                        const float d = v[q][k][e] - mean;
+                        s = fmaf(d, d, s);
+                    }
+            const float rstd = 1.0f / sqrtf(row_sum<TPR>(s, box) / n + a.eps);
+            T *y = static_cast<T *>(a.y) + row * a.N;
+#pragma unroll
+            for (int k = 0; k < NV; ++k) {
+                const uint32_t c = (k * TPR + t) * VEC;
+                if (c < a.N) {
+                    float w[VEC], b[VEC];
+                    ln_param<T, VEC>(a.weight, a.param_f32, c, 1.0f, w);
+                    ln_param<T, VEC>(a.bias, a.param_f32, c, 0.0f, b);
+#pragma unroll
+                    for (int e = 0; e < VEC; ++e) w[e] = fmaf((v[q][k][e] - mean) * rstd, w[e], b[e]);
+                    ln_store<T, VEC>(y + c, w);
                 }
-        const float rstd = 1.0f / sqrtf(row_sum<TPR>(s, box) / n + a.eps);
-        T *y = static_cast<T *>(a.y) + row * a.N;
-#pragma unroll
-        for (int k = 0; k < NV; ++k) {
-            const uint32_t c = (k * TPR + t) * VEC;
-            if (c < a.N) {
-                float w[VEC], b[VEC];
-                ln_param<T, VEC>(a.weight, a.param_f32, c, 1.0f, w);
-                ln_param<T, VEC>(a.bias, a.param_f32, c, 0.0f, b);
-#pragma unroll
-                for (int e = 0; e < VEC; ++e) w[e] = fmaf((v[k][e] - mean) * rstd, w[e], b[e]);
-                ln_store<T, VEC>(y + c, w);
             }
-        }
-        if (t == 0 && a.mean) {
-            a.mean[row] = mean;
-            a.rstd[row] = rstd;
+            if (t == 0 && a.mean) {
+                a.mean[row] = mean;
+                a.rstd[row] = rstd;
+            }
         }
     }
 }
@@ -191,12 +208,12 @@ __global__ __launch_bounds__(256) void k_layer_norm_long(LnArgs a) {
 }
 
 // dx of every row, and this workgroup's share of dw and db: a thread keeps the sums of its own columns over all its rows
-template <typename T, int VEC, int TPR, int NV>
+template <typename T, int VEC, int TPR, int NV, int R>
 __global__ __launch_bounds__(256) void k_layer_norm_bwd(LnArgs a) {
     __shared__ float box[4];
     extern __shared__ float cols[];                    // TPR == 64: [2][N], the wavefronts' sums one after the other
     constexpr int RPW = 256 / TPR;
-    const uint32_t t = threadIdx.x % TPR, sub = threadIdx.x / TPR;
+    const uint32_t t = threadIdx.x % TPR, sub = TPR == 64 ? (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x / TPR)) : 0;
     const float n = (float)a.N;
     float w[NV][VEC], dw[NV][VEC], db[NV][VEC];
 #pragma unroll
@@ -206,42 +223,55 @@ __global__ __launch_bounds__(256) void k_layer_norm_bwd(LnArgs a) {
 #pragma unroll
         for (int e = 0; e < VEC; ++e) dw[k][e] = db[k][e] = 0.0f;
     }
-    for (uint64_t row0 = (uint64_t)blockIdx.x * RPW; row0 < a.M; row0 += (uint64_t)gridDim.x * RPW) {
-        const uint64_t row = row0 + sub;
-        if (TPR == 64 && row >= a.M) break;
-        const T *x = static_cast<const T *>(a.x) + (int64_t)row * a.xs, *dy = static_cast<const T *>(a.dy) + (int64_t)row * a.dys;
-        const float mean = a.mean[row], rstd = a.rstd[row];
-        float xh[NV][VEC], g[NV][VEC];
-        float s0 = 0.0f, s1 = 0.0f;
+    for (uint64_t row0 = ((uint64_t)blockIdx.x * RPW + sub) * R; row0 < a.M; row0 += (uint64_t)gridDim.x * RPW * R) {      // (TPR 256: the same in all threads)
+        float xs[R][NV][VEC], gs[R][NV][VEC], means[R], rstds[R];
 #pragma unroll
-        for (int k = 0; k < NV; ++k) {
-            const uint32_t c = (k * TPR + t) * VEC;
-            if (c < a.N) {
-                ln_load<T, VEC>(x + c, xh[k]);
-                ln_load<T, VEC>(dy + c, g[k]);
-#pragma unroll
-                for (int e = 0; e < VEC; ++e) {
-                    xh[k][e] = (xh[k][e] - mean) * rstd;
-                    db[k][e] += g[k][e];
-                    dw[k][e] = fmaf(g[k][e], xh[k][e], dw[k][e]);
-                    g[k][e] *= w[k][e];
-                    s0 += g[k][e];
-                    s1 = fmaf(g[k][e], xh[k][e], s1);
-                }
-            }
-        }
-        if (a.y) {
-            s0 = row_sum<TPR>(s0, box) / n;
-            s1 = row_sum<TPR>(s1, box) / n;
-            T *dx = static_cast<T *>(a.y) + row * a.N;
+        for (int q = 0; q < R; ++q) {
+            const uint64_t row = row0 + q < a.M ? row0 + q : a.M - 1;
+            const T *x = static_cast<const T *>(a.x) + (int64_t)row * a.xs, *dy = static_cast<const T *>(a.dy) + (int64_t)row * a.dys;
+            means[q] = a.mean[row];
+            rstds[q] = a.rstd[row];
 #pragma unroll
             for (int k = 0; k < NV; ++k) {
                 const uint32_t c = (k * TPR + t) * VEC;
                 if (c < a.N) {
-                    float o[VEC];
+                    ln_load<T, VEC>(x + c, xs[q][k]);
+                    ln_load<T, VEC>(dy + c, gs[q][k]);
+                }
+            }
+        }
 #pragma unroll
-                    for (int e = 0; e < VEC; ++e) o[e] = rstd * (g[k][e] - s0 - xh[k][e] * s1);
-                    ln_store<T, VEC>(dx + c, o);
+        for (int q = 0; q < R; ++q) {
+            const uint64_t row = row0 + q;
+            if (row >= a.M) break;
+            const float mean = means[q], rstd = rstds[q];
+            float(&xh)[NV][VEC] = xs[q], (&g)[NV][VEC] = gs[q];
+            float s0 = 0.0f, s1 = 0.0f;
+#pragma unroll
+            for (int k = 0; k < NV; ++k)
+                if ((k * TPR + t) * VEC < a.N)
+#pragma unroll
+                    for (int e = 0; e < VEC; ++e) {
+                        xh[k][e] = (xh[k][e] - mean) * rstd;
+                        db[k][e] += g[k][e];
+                        dw[k][e] = fmaf(g[k][e], xh[k][e], dw[k][e]);
+                        g[k][e] *= w[k][e];
+                        s0 += g[k][e];
+                        s1 = fmaf(g[k][e], xh[k][e], s1);
+                    }
+            if (a.y) {
+                s0 = row_sum<TPR>(s0, box) / n;
+                s1 = row_sum<TPR>(s1, box) / n;
+                T *dx = static_cast<T *>(a.y) + row * a.N;
+#pragma unroll
+                for (int k = 0; k < NV; ++k) {
+                    const uint32_t c = (k * TPR + t) * VEC;
+                    if (c < a.N) {
+                        float o[VEC];
+#pragma unroll
+                        for (int e = 0; e < VEC; ++e) o[e] = rstd * (g[k][e] - s0 - xh[k][e] * s1);
+                        ln_store<T, VEC>(dx + c, o);
+                    }
                 }
             }
         }
@@ -346,8 +376,17 @@ __global__ __launch_bounds__(1024) void k_layer_norm_cols(const float *__restric
     __shared__ float s[32][33];
     const uint32_t c = blockIdx.x * 32 + (threadIdx.x & 31), r0 = threadIdx.x >> 5;
     float acc = 0.0f;
-    if (c < 2 * N)
-        for (uint32_t r = r0; r < rows; r += 32) acc += partial[(uint64_t)r * 2 * N + c];
+    if (c < 2 * N) {
+        uint32_t r = r0;
+        for (; r + 7 * 32 < rows; r += 8 * 32) {               // (eight loads in flight)
+            float v[8];
+#pragma unroll
+            for (int x = 0; x < 8; ++x) v[x] = partial[(uint64_t)(r + x * 32) * 2 * N + c];
+#pragma unroll
+            for (int x = 0; x < 8; ++x) acc += v[x];
+        }
+        for (; r < rows; r += 32) acc += partial[(uint64_t)r * 2 * N + c];
+    }
     s[r0][threadIdx.x & 31] = acc;
     __syncthreads();
     // 32 columns x 32 partial sums: the wavefronts read them transposed, 32 lanes per column
@@ -376,15 +415,17 @@ static bool ln_aligned(const void *p, int64_t pitch, size_t size) { return ((uin
 
 template <typename T, int VEC>
 static void ln_forward(const LnArgs &a, hipStream_t st) {
-    const uint64_t waves = (a.M + 3) / 4, most = 1u << 22;
+    const uint64_t most = 1u << 22, waves = (a.M + 3) / 4;
     const uint32_t g4 = (uint32_t)(waves < most ? waves : most), g1 = (uint32_t)(a.M < most ? a.M : most);
     constexpr int E = VEC == 1 ? 8 : VEC;              // elements of a "step" per thread
     constexpr int S = E / VEC;                         // vectors per step
-    if (a.N <= 64u * E) k_layer_norm<T, VEC, 64, S><<<g4, 256, 0, st>>>(a);
-    else if (a.N <= 128u * E) k_layer_norm<T, VEC, 64, 2 * S><<<g4, 256, 0, st>>>(a);
-    else if (a.N <= 256u * E) k_layer_norm<T, VEC, 256, S><<<g1, 256, 0, st>>>(a);
-    else if (a.N <= 512u * E) k_layer_norm<T, VEC, 256, 2 * S><<<g1, 256, 0, st>>>(a);
-    else if (a.N <= 1024u * E) k_layer_norm<T, VEC, 256, 4 * S><<<g1, 256, 0, st>>>(a);
+    constexpr int MANY = VEC == 1 ? 1 : 4;             // rows of a wavefront at a time where there are rows for every wavefront of the chip
+    const bool many = a.M >= (uint64_t)cu_count() * 64;
+    if (a.N <= 64u * E) many ? k_layer_norm<T, VEC, 64, S, MANY><<<div_up(g4, MANY), 256, 0, st>>>(a) : k_layer_norm<T, VEC, 64, S, 1><<<g4, 256, 0, st>>>(a);
+    else if (a.N <= 128u * E) many ? k_layer_norm<T, VEC, 64, 2 * S, (MANY + 1) / 2><<<div_up(g4, (MANY + 1) / 2), 256, 0, st>>>(a) : k_layer_norm<T, VEC, 64, 2 * S, 1><<<g4, 256, 0, st>>>(a);
+    else if (a.N <= 256u * E) k_layer_norm<T, VEC, 256, S, 1><<<g1, 256, 0, st>>>(a);
+    else if (a.N <= 512u * E) k_layer_norm<T, VEC, 256, 2 * S, 1><<<g1, 256, 0, st>>>(a);
+    else if (a.N <= 1024u * E) k_layer_norm<T, VEC, 256, 4 * S, 1><<<g1, 256, 0, st>>>(a);
     else k_layer_norm_long<T, VEC><<<g1, 256, 0, st>>>(a);
 }
 
@@ -392,10 +433,12 @@ template <typename T, int VEC>
 static void ln_backward(const LnArgs &a, uint32_t groups, hipStream_t st) {
     constexpr int E = VEC == 1 ? 8 : VEC, S = E / VEC;
     const uint32_t lds = a.partial ? 2 * a.N * 4 : 0;
-    if (a.N <= 64u * E) k_layer_norm_bwd<T, VEC, 64, S><<<groups, 256, lds, st>>>(a);
-    else if (a.N <= 128u * E) k_layer_norm_bwd<T, VEC, 64, 2 * S><<<groups, 256, lds, st>>>(a);
-    else if (a.N <= 256u * E) k_layer_norm_bwd<T, VEC, 256, S><<<groups, 256, 0, st>>>(a);
-    else if (a.N <= 512u * E) k_layer_norm_bwd<T, VEC, 256, 2 * S><<<groups, 256, 0, st>>>(a);
+    constexpr int MANY = VEC == 1 ? 1 : 4;             // (as in the forward pass)
+    const bool many = a.M >= (uint64_t)cu_count() * 64;
+    if (a.N <= 64u * E) many ? k_layer_norm_bwd<T, VEC, 64, S, MANY><<<groups, 256, lds, st>>>(a) : k_layer_norm_bwd<T, VEC, 64, S, 1><<<groups, 256, lds, st>>>(a);
+    else if (a.N <= 128u * E) many ? k_layer_norm_bwd<T, VEC, 64, 2 * S, (MANY + 1) / 2><<<groups, 256, lds, st>>>(a) : k_layer_norm_bwd<T, VEC, 64, 2 * S, 1><<<groups, 256, lds, st>>>(a);
+    else if (a.N <= 256u * E) k_layer_norm_bwd<T, VEC, 256, S, 1><<<groups, 256, 0, st>>>(a);
+    else if (a.N <= 512u * E) k_layer_norm_bwd<T, VEC, 256, 2 * S, 1><<<groups, 256, 0, st>>>(a);
     else {
         const uint64_t most = 1u << 22;
         if (a.y) k_layer_norm_bwd_long<T, VEC><<<(uint32_t)(a.M < most ? a.M : most), 256, 0, st>>>(a);
