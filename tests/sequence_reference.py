@@ -13,16 +13,16 @@ def u(dtype):
     return torch.finfo(dtype).eps / 2
 
 
-def visible(n_q, n_k, q_start, left, right, sinks, n):
+def visible(n_q, n_k, q_start, left, right, sinks, n, device="cpu"):
     """[n_q, n_k] bool: what query i (position q_start + i) of a sequence of n tokens sees; None: no end."""
-    p, j = q_start + torch.arange(n_q)[:, None], torch.arange(n_k)[None, :]
-    near = torch.ones(n_q, n_k, dtype=torch.bool) if left is None else (j >= p - left)
-    ahead = torch.ones(n_q, n_k, dtype=torch.bool) if right is None else (j <= p + right)
+    p, j = q_start + torch.arange(n_q, device=device)[:, None], torch.arange(n_k, device=device)[None, :]
+    near = torch.ones(n_q, n_k, dtype=torch.bool, device=device) if left is None else (j >= p - left)
+    ahead = torch.ones(n_q, n_k, dtype=torch.bool, device=device) if right is None else (j <= p + right)
     return ahead & (near | (j < sinks)) & (j < n) & (p < n)
 
 
 def attention(q, k, v, dout=None, left=None, right=0, sinks=0, lengths=None, scale=None, q_start=None):
-    """{name: (value, bound)} of out and, with dout, dq, dk, dv; inputs [B, T, H, D] of any type, on the CPU."""
+    """{name: (value, bound)} of out and, with dout, dq, dk, dv; inputs [B, T, H, D] of any type; computed where they are."""
     dtype = q.dtype
     r = u(dtype) if dtype != torch.float32 else 0.0            # (32 bits: the matrix products take their operands as they are)
     ro = u(dtype)
@@ -37,12 +37,13 @@ def attention(q, k, v, dout=None, left=None, right=0, sinks=0, lengths=None, sca
     bnd = {n: torch.zeros_like(t) for n, t in val.items()}
     for b in range(B):
         n = Tk if lengths is None else max(0, min(int(lengths[b]), Tk))
-        see = visible(Tq, Tk, q_start, left, right, sinks, n)
+        see = visible(Tq, Tk, q_start, left, right, sinks, n, q.device)
+        inside_q, inside_k = ((start + torch.arange(t, device=q.device) < n)[:, None] for start, t in ((q_start, Tq), (0, Tk)))
         rows = see.any(1)
         for h in range(Hq):
             # what lies behind the sequence may hold anything: it is not part of the definition
-            qh = torch.where((q_start + torch.arange(Tq) < n)[:, None], q[b, :, h], 0.0)
-            kh, vh = (torch.where((torch.arange(Tk) < n)[:, None], t[b, :, h // G], 0.0) for t in (k, v))
+            qh = torch.where(inside_q, q[b, :, h], 0.0)
+            kh, vh = (torch.where(inside_k, t[b, :, h // G], 0.0) for t in (k, v))
             s = (qh @ kh.T) * scale
             P = torch.softmax(torch.where(see, s, -math.inf), 1)
             P = torch.where(rows[:, None], P, 0.0)
@@ -57,7 +58,7 @@ def attention(q, k, v, dout=None, left=None, right=0, sinks=0, lengths=None, sca
             val["out"][b, :, h], bnd["out"][b, :, h] = o, ro * o.abs() + eo * (1 + ro)
             if dout is None:
                 continue
-            g = torch.where((q_start + torch.arange(Tq) < n)[:, None], dout[b, :, h].double(), 0.0)
+            g = torch.where(inside_q, dout[b, :, h].double(), 0.0)
             dP = g @ vh.T
             delta = (g * o).sum(1, keepdim=True)
             dS = P * (dP - delta)
@@ -141,7 +142,7 @@ def rotary(x, positions, frequencies, sections, interleaved=False, backward=Fals
 
 def close(got, value_bound, name):
     value, bound = value_bound
-    got = got.detach().double().cpu()
+    got = got.detach().double().to(value.device)
     assert got.shape == value.shape, (name, got.shape, value.shape)
     assert torch.isfinite(got).all(), f"{name}: not finite"
     off = (got - value).abs() - bound

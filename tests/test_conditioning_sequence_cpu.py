@@ -47,7 +47,8 @@ def test_rotary_refusals():
                         (dict(x=(x, x, x)), "one tensor or two"), (dict(sections=(3, 6), frequencies=z(9, dtype=f64)), "sections"), (dict(sections=()), "sections"),
                         (dict(sections=(-1, 9)), "sections"), (dict(sections=(1, 1, 1, 1, 4)), "sections"), (dict(positions=z(3, 2, dtype=f64)), "positions"),
                         (dict(positions=z(3)), "positions"), (dict(positions=z(1, 3, 2)), "positions"), (dict(frequencies=z(8)), "frequencies"),
-                        (dict(frequencies=z(7, dtype=f64)), "frequencies"), (dict(x=x.double()), "float32, float16 or bfloat16")):
+                        (dict(frequencies=z(7, dtype=f64)), "frequencies"), (dict(x=x.double()), "float32, float16 or bfloat16"), (dict(frequencies=z(8, dtype=f64).requires_grad_(True)), "no gradient"),
+                        (dict(positions=z(3, 2).requires_grad_(True)), "no gradient")):
         with pytest.raises(GfppError, match=why):
             rotary_embed(**{**ok, **change})
     with pytest.raises(GfppError, match="sections"):

@@ -84,6 +84,20 @@ def test_layer_norm_large_offset_keeps_its_spread():
     ref.close(layer_norm(x.cuda()), ref.layer_norm(x, None, None, 1e-5)["y"], "y")
 
 
+@pytest.mark.parametrize("dtype,N", [(torch.float32, 204), (torch.float32, 300), (torch.bfloat16, 1000), (torch.float16, 24), (torch.float16, 31)])
+def test_layer_norm_many_rows(dtype, N):
+    """Rows for every wavefront of the chip: several rows of a wavefront in flight, a last share that is not whole."""
+    M = 64 * torch.cuda.get_device_properties(0).multi_processor_count + 3
+    g = gen(N)
+    x, w, b, dy = (rand(g, M, N, scale=2.0) + 1.0).to(dtype), rand(g, N, mean=1.0), rand(g, N), rand(g, M, N, dtype=dtype)
+    want = ref.layer_norm(x, w, b, 1e-5, dy)
+    leaves = [t.cuda().requires_grad_(True) for t in (x, w, b)]
+    y = layer_norm(*leaves)
+    ref.close(y, want["y"], "y")
+    for name, got in zip(("dx", "dweight", "dbias"), torch.autograd.grad(y, leaves, dy.cuda())):
+        ref.close(got, want[name], name)
+
+
 # ---- rotary positions ------------------------------------------------------------------------------------------------------------------------------------
 @pytest.mark.parametrize("dtype", TYPES, ids=IDS)
 @pytest.mark.parametrize("interleaved", [False, True])
@@ -269,6 +283,55 @@ def test_attention_sinks_of_a_long_sequence(dtype, D):
         again = run_attention(*dev, **how)
         for n in got:
             assert torch.equal(got[n], again[n]), n
+
+
+@pytest.mark.parametrize("dtype,B,Hq,Hk,D,left,right,sinks", [
+    (torch.bfloat16, 4, 16, 4, 128, 150, 20, 3),           # two heads of a group a workgroup
+    (torch.float16, 4, 16, 16, 120, 90, 0, 2),             # 128 keys a workgroup in the backward pass
+    (torch.bfloat16, 4, 16, 16, 64, 300, 0, 0), (torch.float32, 4, 16, 16, 40, 100, 10, 1), (torch.float32, 4, 16, 16, 96, 100, 10, 1),
+    (torch.bfloat16, 4, 16, 2, 64, 20, 11, 2), (torch.float16, 4, 16, 8, 33, 10, 0, 0), (torch.float32, 4, 16, 4, 32, 7, 8, 4)])      # few keys and a large grid
+def test_attention_grids_that_fill_the_chip(dtype, B, Hq, Hk, D, left, right, sinks):
+    """The variants that large grids take; the definition in 64 bits is computed on the GPU here."""
+    T = 1100
+    q, k, v, dout = (t.cuda() for t in attention_inputs(D, B, T, T, Hq, Hk, D, dtype))
+    assert -(-T // 128) * Hq * B >= 2 * torch.cuda.get_device_properties(0).multi_processor_count
+    lengths = (T, T - 1, 700, 5)
+    how = dict(left=left, right=right, sinks=sinks)
+    want = ref.attention(q, k, v, dout, lengths=lengths, **how)
+    got = run_attention(q, k, v, dout, lengths=torch.tensor(lengths, dtype=torch.int32).cuda(), **how)
+    for n in got:
+        ref.close(got[n], want[n], n)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS)
+def test_attention_far_offsets(dtype):
+    """A view into a batch whose heads lie more than 2^31 elements apart, and rows so far apart that 64 of them span more than 2^31 bytes."""
+    T, D = 40, 64
+    q, k, v, dout = attention_inputs(5, 1, T, T, 2, 2, D, dtype)
+    want = run_attention(*(t.cuda() for t in (q, k, v, dout)), left=9)
+    room = torch.empty(2 ** 31 + 2 ** 22, dtype=dtype, device="cuda")
+    apart = torch.as_strided(room, (1, T, 2, D), (0, 2 * D, 2 ** 31 + 64, 1))
+    apart.copy_(k.cuda())
+    rows = torch.as_strided(room, (1, T, 2, D), (0, 2 ** 25, D, 1), 2 ** 21)
+    got = run_attention(q.cuda(), apart, v.cuda(), dout.cuda(), left=9)
+    for n in want:
+        assert torch.equal(got[n], want[n]), n
+    rows.copy_(v.cuda())
+    got = run_attention(q.cuda(), k.cuda(), rows, dout.cuda(), left=9)
+    for n in want:
+        assert torch.equal(got[n], want[n]), n
+
+
+def test_other_device():
+    """Tensors of another GPU than the current one."""
+    if torch.cuda.device_count() < 2:
+        pytest.skip("one GPU")
+    q, k, v, dout = attention_inputs(1, 1, 50, 50, 2, 1, 32, torch.bfloat16)
+    want = run_attention(*(t.cuda() for t in (q, k, v, dout)), left=9)
+    got = run_attention(*(t.to("cuda:1") for t in (q, k, v, dout)), left=9)
+    assert torch.cuda.current_device() == 0
+    for n in want:
+        assert torch.equal(got[n].cpu(), want[n].cpu()), n
 
 
 def test_attention_gradient_against_differences():
