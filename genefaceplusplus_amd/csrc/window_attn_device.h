@@ -93,7 +93,8 @@ struct WaStage {
         const int row = (int)threadIdx.x / PER_ROW, col = (int)threadIdx.x % PER_ROW * V;
         if constexpr (VEC) {
             const int rows = end - r0 < ROWS ? (end - r0 > 0 ? end - r0 : 0) : ROWS, pitch = (int)stride * (int)sizeof(T);
-            const auto rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<T *>(tile), 0, rows * pitch, 0x00020000);
+            // (a scalar by its making: the compiler clamps in the vector unit and would then load lane group by lane group)
+            const auto rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<T *>(tile), 0, __builtin_amdgcn_readfirstlane(rows * pitch), 0x00020000);
             const uint32_t at = col < D && (ALL >= THREADS || (int)threadIdx.x < ALL) ? (uint32_t)(row * pitch + col * (int)sizeof(T)) : 0x7ffffff0u;
 #pragma unroll
             for (int n = 0; n < N; ++n)                        // (the whole offset in the lane: the range check subtracts a scalar offset from the size, without a sign)
