@@ -55,34 +55,27 @@ __global__ __launch_bounds__(64 * WAVES * HEADS, WAVES == 1 ? 1 : (sizeof(T) == 
     // two tiles in flight: the one that the next step stores and the one after it (one alone arrives later than the step that it was requested in takes)
     WaStage<T, DP, BN, VEC, 64 * WAVES * HEADS> rk[2], rv[2];
     auto tile_row = [&](int k) { return (k < range.head ? k : range.lo + k - range.head) * BN; };
-    if (tiles > 0) {
-        rk[0].load(kb, a.k.st, tile_row(0), n, a.D);
-        rv[0].load(vb, a.v.st, tile_row(0), n, a.D);
-        if (tiles > 1) {
-            rk[1].load(kb, a.k.st, tile_row(1), n, a.D);
-            rv[1].load(vb, a.v.st, tile_row(1), n, a.D);
-        }
-        rk[0].store(s_k[0], PK);
-        rv[0].store(s_v[0], PV);
-        if (tiles > 2) {
-            rk[0].load(kb, a.k.st, tile_row(2), n, a.D);
-            rv[0].load(vb, a.v.st, tile_row(2), n, a.D);
-        }
-    }
+    // Loads and stores of tiles are unconditional -- past the last tile a load's range is empty, nothing is read --: a load behind a branch may or may not be in flight, and
+    // every wait would then be for all of them.
+    auto load = [&](int which, int k) {
+        const int r0 = k < tiles ? tile_row(k) : (n > 0 ? n : 0);
+        rk[which].load(kb, a.k.st, r0, n, a.D);
+        rv[which].load(vb, a.v.st, r0, n, a.D);
+    };
+    load(0, 0);
+    load(1, 1);
+    rk[0].store(s_k[0], PK);
+    rv[0].store(s_v[0], PV);
+    load(0, 2);
     wa_arrived(q);
     __syncthreads();
     const int row_at = c * PK + 8 * h * (int)sizeof(T), col_at = wa_col_offset<T>(lane, PV);
     auto step = [&](int k, auto which) {
         constexpr int buf = decltype(which)::value, other = buf ^ 1;     // of tile k (LDS) and of tile k + 1 (LDS, registers)
         const int j0 = tile_row(k), j1 = j0 + BN - 1;
-        if (k + 1 < tiles) {
-            rk[other].store(s_k[other], PK);                     // (last read before the previous barrier)
-            rv[other].store(s_v[other], PV);
-            if (k + 3 < tiles) {
-                rk[other].load(kb, a.k.st, tile_row(k + 3), n, a.D);
-                rv[other].load(vb, a.v.st, tile_row(k + 3), n, a.D);
-            }
-        }
+        rk[other].store(s_k[other], PK);                         // (last read before the previous barrier)
+        rv[other].store(s_v[other], PV);
+        load(other, k + 3);
         const bool seen = pw0 < n && j0 <= pw1 + a.right && (j1 >= pw0 - a.left || j0 < a.sinks);
         if (seen) {
             v16f s[NSUB];
@@ -158,9 +151,10 @@ __global__ __launch_bounds__(64 * WAVES * HEADS, WAVES == 1 ? 1 : (sizeof(T) == 
         }
         __syncthreads();
     };
-    for (int k = 0; k < tiles; k += 2) {
+    for (int k = 0; k < tiles; ++k) {
         step(k, WaInt<0>{});
-        if (k + 1 < tiles) step(k + 1, WaInt<1>{});
+        if (++k >= tiles) break;                               // (no way from an even step to the next even one: what is in flight is the same at every wait)
+        step(k, WaInt<1>{});
     }
     l = half_wave_sum(l);
     if (i >= a.Tq) return;

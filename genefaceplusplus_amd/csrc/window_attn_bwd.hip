@@ -74,20 +74,18 @@ __global__ __launch_bounds__(kWaThreads * HEADS, sizeof(T) == 2 && (VEC || DP <=
     // two tiles in flight: the one that the next step stores and the one after it (one alone arrives later than the step that it was requested in takes)
     WaStage<T, DP, BN, VEC, kWaThreads * HEADS> rk[2], rv[2];
     auto tile_row = [&](int k) { return (k < range.head ? k : range.lo + k - range.head) * BN; };
-    if (tiles > 0) {
-        rk[0].load(kb, a.k.st, tile_row(0), n, a.D);
-        rv[0].load(vb, a.v.st, tile_row(0), n, a.D);
-        if (tiles > 1) {
-            rk[1].load(kb, a.k.st, tile_row(1), n, a.D);
-            rv[1].load(vb, a.v.st, tile_row(1), n, a.D);
-        }
-        rk[0].store(s_k[0], PK);
-        rv[0].store(s_v[0], PV);
-        if (tiles > 2) {
-            rk[0].load(kb, a.k.st, tile_row(2), n, a.D);
-            rv[0].load(vb, a.v.st, tile_row(2), n, a.D);
-        }
-    }
+    // Loads and stores of tiles are unconditional -- past the last tile a load's range is empty, nothing is read --: a load behind a branch may or may not be in flight, and
+    // every wait would then be for all of them.
+    auto load = [&](int which, int k) {
+        const int r0 = k < tiles ? tile_row(k) : (n > 0 ? n : 0);
+        rk[which].load(kb, a.k.st, r0, n, a.D);
+        rv[which].load(vb, a.v.st, r0, n, a.D);
+    };
+    load(0, 0);
+    load(1, 1);
+    rk[0].store(s_k[0], PK);
+    rv[0].store(s_v[0], PV);
+    load(0, 2);
     wa_arrived(q);
     wa_arrived(g);
     __syncthreads();
@@ -95,14 +93,9 @@ __global__ __launch_bounds__(kWaThreads * HEADS, sizeof(T) == 2 && (VEC || DP <=
     auto step = [&](int k, auto which) {
         constexpr int buf = decltype(which)::value, other = buf ^ 1;
         const int j0 = tile_row(k), j1 = j0 + BN - 1;
-        if (k + 1 < tiles) {
-            rk[other].store(s_k[other], PK);
-            rv[other].store(s_v[other], PV);
-            if (k + 3 < tiles) {
-                rk[other].load(kb, a.k.st, tile_row(k + 3), n, a.D);
-                rv[other].load(vb, a.v.st, tile_row(k + 3), n, a.D);
-            }
-        }
+        rk[other].store(s_k[other], PK);                         // (last read before the previous barrier)
+        rv[other].store(s_v[other], PV);
+        load(other, k + 3);
         const bool seen = pw0 < n && j0 <= pw1 + a.right && (j1 >= pw0 - a.left || j0 < a.sinks);
         if (seen) {
             const bool full = pw1 < n && j1 < n && j1 <= pw0 + a.right && (j0 >= pw1 - a.left || j1 < a.sinks);
@@ -141,9 +134,10 @@ __global__ __launch_bounds__(kWaThreads * HEADS, sizeof(T) == 2 && (VEC || DP <=
         }
         __syncthreads();
     };
-    for (int k = 0; k < tiles; k += 2) {
+    for (int k = 0; k < tiles; ++k) {
         step(k, WaInt<0>{});
-        if (k + 1 < tiles) step(k + 1, WaInt<1>{});
+        if (++k >= tiles) break;                               // (no way from an even step to the next even one: what is in flight is the same at every wait)
+        step(k, WaInt<1>{});
     }
     if (i < a.Tq) wa_store_rows<T, NT, VEC>(acc, a.scale, static_cast<T *>(a.dq.p) + b * a.dq.sb + (int64_t)i * a.dq.st + hq * a.dq.sh, h, a.D);
 }
@@ -200,18 +194,21 @@ __global__ __launch_bounds__(PAIRS * 128, PAIRS == 2 && DP == 128 && (sizeof(T) 
     }
     const int steps = tiles * a.G;
     WaStage<T, DP, BQ, VEC, PAIRS * 128> rq[2], rg[2];                                 // two tiles in flight (k_window_attn)
-    float r_stat[2] = {0.0f, 0.0f};
-    int next_tile = 0, next_head = 0;                                                  // of the tile that is loaded next: the heads of a group one after the other
+    float r_lse[2], r_delta[2];
+    int next_tile = 0, next_head = 0, loaded = 0;                                      // of the tile that is loaded next: the heads of a group one after the other
+    // (unconditional, as in the forward pass: past the last tile the ranges are empty)
     auto load = [&](int which) {
-        const int hq = hk * a.G + next_head, i = i_lo + next_tile * BQ;
+        const bool more = loaded < steps;
+        const int hq = hk * a.G + (more ? next_head : 0), i = more ? i_lo + next_tile * BQ : (end > 0 ? end : 0);
         rq[which].load(static_cast<const T *>(a.q.p) + b * a.q.sb + hq * a.q.sh, a.q.st, i, end, a.D);
         rg[which].load(static_cast<const T *>(a.dout.p) + b * a.dout.sb + hq * a.dout.sh, a.dout.st, i, end, a.D);
-        if (threadIdx.x < 2 * BQ) {
-            const int row = i + (int)(threadIdx.x % BQ);
-            const int64_t at = ((int64_t)b * a.Hq + hq) * a.Tq + row;
-            if (threadIdx.x < BQ) r_stat[which] = row < end ? a.lse[at] : INFINITY;
-            else r_stat[which] = row < end ? a.delta[at] : 0.0f;
-        }
+        const int64_t at = ((int64_t)b * a.Hq + hq) * a.Tq + i;
+        const int rows = __builtin_amdgcn_readfirstlane(end - i < BQ ? (end - i > 0 ? end - i : 0) : BQ);
+        const int off = threadIdx.x < BQ ? (int)threadIdx.x * 4 : 0x7ffffff0;
+        r_lse[which] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(__builtin_amdgcn_make_buffer_rsrc(a.lse + at, 0, rows * 4, 0x00020000), off, 0, 0));
+        r_delta[which] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(__builtin_amdgcn_make_buffer_rsrc(a.delta + at, 0, rows * 4, 0x00020000), off, 0, 0));
+        if ((int)threadIdx.x >= rows) r_lse[which] = INFINITY;                         // rows behind the sequence: probability 0
+        ++loaded;
         if (++next_tile == tiles) {
             next_tile = 0;
             ++next_head;
@@ -220,15 +217,15 @@ __global__ __launch_bounds__(PAIRS * 128, PAIRS == 2 && DP == 128 && (sizeof(T) 
     auto store = [&](int buf, int which) {
         rq[which].store(s_q[buf], PITCH);
         rg[which].store(s_g[buf], PITCH);
-        if (threadIdx.x < BQ) s_lse[buf][threadIdx.x] = r_stat[which];
-        else if (threadIdx.x < 2 * BQ) s_delta[buf][threadIdx.x - BQ] = r_stat[which];
+        if (threadIdx.x < BQ) {
+            s_lse[buf][threadIdx.x] = r_lse[which];
+            s_delta[buf][threadIdx.x] = r_delta[which];
+        }
     };
-    if (steps > 0) {
-        load(0);
-        if (steps > 1) load(1);
-        store(0, 0);
-        if (steps > 2) load(0);
-    }
+    load(0);
+    load(1);
+    store(0, 0);
+    load(0);
     wa_arrived(f);
     __syncthreads();
     const int row_at = c * PITCH + 8 * h * (int)sizeof(T), col_at = wa_col_offset<T>(lane, PITCH);
@@ -237,10 +234,8 @@ __global__ __launch_bounds__(PAIRS * 128, PAIRS == 2 && DP == 128 && (sizeof(T) 
     auto step = [&](int k, auto parity) {
         constexpr int odd = decltype(parity)::value;                                   // k & 1; tile k + 1 is in the other registers
         const int next = now == 2 ? 0 : now + 1;
-        if (k + 1 < steps) {
-            store(next, odd ^ 1);                                                      // (tile k - 2's: last read a step ago, before the barrier)
-            if (k + 3 < steps) load(odd ^ 1);
-        }
+        store(next, odd ^ 1);                                                          // (tile k - 2's: last read a step ago, before the barrier)
+        load(odd ^ 1);
         const int p0 = a.q_start + i_lo + tile * BQ, p1 = p0 + BQ - 1;
         const bool seen = jw0 < n && p1 >= jw0 - a.right && (p0 <= jw1 + a.left || jw0 < a.sinks);
         if (!second) {
