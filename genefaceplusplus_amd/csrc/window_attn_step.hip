@@ -9,6 +9,8 @@
 // fourth tile of 32 slots of its workgroup's stretch, the next tile in flight in registers; the four partial softmaxes meet in LDS.  Few streams: the
 // slots of a stream are split over several workgroups, whose partial results a second launch joins.
 // Probabilities enter the products as a rounded value and its rounded remainder, so that the output carries its own rounding alone.
+// Measured (bf16): 64 streams x 32 heads on 8 x 128, 4 100 slots (1.08 GB): 206 us with the join, 5.2 TB/s, what a copy of 2 GiB reaches; one stream x 8 on 2 x 64, 260 slots:
+// 6.3 us, a launch's latency and four dependent trips to memory.  One element at a time (unaligned rows) takes 1 000 and 23 us.
 // The row of the new token is taken from the arguments by whoever reads that slot, and written by one wavefront: no order between workgroups is needed.
 #include "window_attn_device.h"
 
@@ -35,11 +37,13 @@ __global__ __launch_bounds__(kWaThreads, sizeof(T) == 2 ? 2 : 1) void k_window_a
     constexpr int TILES = 4 * 32 * PV, RESULTS = 4 * 32 * (DP + 4) * 4;
     __shared__ __attribute__((aligned(16))) unsigned char lds[TILES > RESULTS ? TILES : RESULTS];
     __shared__ float s_m[4][32], s_l[4][32];
+    // Consecutive workgroups go to the 8 XCDs in turn.  Heads taken in order would give an XCD the same few heads of every stream, whose rows, a whole token apart, lie on
+    // the same few channels of its L2; turned by the stretch and the stream, every XCD sees all of them (64 streams x 8 heads x 128, 4 100 slots in 4 stretches: 227 -> 206 us).
     const uint32_t split = blockIdx.x % a.splits;
     uint32_t item = blockIdx.x / a.splits;
     const int chunk = (int)(item % a.chunks);
     item /= a.chunks;
-    const int hk = (int)(item % a.Hk), b = (int)(item / a.Hk);
+    const int b = (int)(item / a.Hk), hk = (int)((item % a.Hk + split + b) % a.Hk);
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = lane & 31, h = lane >> 5;
     const int64_t n = a.pos64 ? static_cast<const int64_t *>(a.pos)[b] : (int64_t)static_cast<const int32_t *>(a.pos)[b];
     const int window = a.slots - a.sinks;
@@ -208,13 +212,16 @@ static void ws_launch(const WsArgs &a, bool vec, uint32_t grid, hipStream_t st) 
     if (a.splits > 1) k_window_attn_step_join<T><<<(uint32_t)a.B * a.Hq, 128, 0, st>>>(a);
 }
 
-// stretches of a stream's slots: enough workgroups for four per CU, at least 512 slots (four tiles per wavefront) each: below, the second launch costs what the
-// stretches save
+// Stretches that a stream's slots are cut into, us measured with 8 key heads of 128 features, 4 100 slots.
+// Groups (of query heads that share keys) for half the CUs at most: one workgroup per CU (4 streams: 88 whole, 28 in 8 stretches; 16 streams: 97 and 65 in 2), of 320
+// slots at least -- below, the second launch costs what the stretches save (1 stream, 64 features, 516 slots: 8.4 whole, 9.0 in 2; 1 028 slots: 11.5 whole, 10.1 in 3).
+// More groups: five stretches, so that one workgroup's start and end lie under the loads of others (64 streams: 219 whole, 204 in 5, 221 in 12), of 768 slots at least
+// (32 streams x 8 heads x 64, 1 028 slots: 22 whole, 26 in 2).  The one size in between that would rather stay whole is one group per CU (107, 114 in 5).
 static uint32_t ws_splits(uint32_t B, uint32_t Hq, uint32_t Hk, uint32_t slots) {
-    const uint64_t groups = (uint64_t)B * Hk * (((uint64_t)Hq / Hk + 31) / 32);
+    const uint64_t groups = (uint64_t)B * Hk * (((uint64_t)Hq / Hk + 31) / 32), cus = (uint64_t)cu_count();
     if (groups == 0) return 1;
-    const uint64_t want = ((uint64_t)cu_count() * 4 + groups - 1) / groups, most = slots / 512;
-    const uint64_t n = want < most ? want : most;
+    const bool few = groups * 2 <= cus;
+    const uint64_t want = few ? (cus + groups - 1) / groups : 5, most = slots / (few ? 320 : 768), n = want < most ? want : most;
     return n < 1 ? 1 : (uint32_t)n;
 }
 
@@ -274,7 +281,7 @@ GFPP_API int gfpp_window_attn_step(const void *q, const void *k, const void *v, 
     a.c = scale * 1.4426950408889634f;
     a.splits = ws_splits(B, Hq, Hk, slots);
     WS_REQUIRE(a.splits == 1 || scratch);
-    a.per_split = (int)(div_up(div_up(slots, a.splits), 128) * 128);
+    a.per_split = (int)(div_up(div_up(slots, a.splits), 32) * 32);
     const uint64_t grid = (uint64_t)B * Hk * a.chunks * a.splits;
     WS_REQUIRE(grid <= 0x7fffffffull && (uint64_t)B * Hq <= 0x7fffffffull);
     const size_t size = dtype == GFPP_F32 ? 4 : 2;
