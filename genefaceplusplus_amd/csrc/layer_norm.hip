@@ -8,6 +8,9 @@
 // elements); longer rows are read again, out of the L2.  Statistics, both row sums of the backward pass and the column sums are fp32 for every type; the outputs
 // are rounded once.  The column sums of dw / db stay in registers over the rows of a workgroup, leave as one partial row per workgroup and are added in a fixed
 // order by a second launch: no atomics, the same bits every time.
+// Measured: 13 000 x 1 024 bf16 with fp32 parameters: forward 12.8 us (53 MB, 4.2 TB/s), backward 21.9 (80 MB, 3.6 TB/s) and 4.0 for the column sums; 65 537 x 204 fp32: forward
+// 24.5 us (107 MB, 4.4 TB/s), backward 28.9 (160 MB, 5.5 TB/s) and 4.0.  Rows that 16-byte vectors do not divide go one element at a time: 24.7 and 36.3, 32.2 and 47.0.
+// One row of 1 024: 2.7 us, a launch.
 #include "gfpp_common.h"
 
 namespace gfpp {
@@ -419,10 +422,13 @@ static void ln_forward(const LnArgs &a, hipStream_t st) {
     const uint32_t g4 = (uint32_t)(waves < most ? waves : most), g1 = (uint32_t)(a.M < most ? a.M : most);
     constexpr int E = VEC == 1 ? 8 : VEC;              // elements of a "step" per thread
     constexpr int S = E / VEC;                         // vectors per step
-    constexpr int MANY = VEC == 1 ? 1 : 4;             // rows of a wavefront at a time where there are rows for every wavefront of the chip
-    const bool many = a.M >= (uint64_t)cu_count() * 64;
-    if (a.N <= 64u * E) many ? k_layer_norm<T, VEC, 64, S, MANY><<<div_up(g4, MANY), 256, 0, st>>>(a) : k_layer_norm<T, VEC, 64, S, 1><<<g4, 256, 0, st>>>(a);
-    else if (a.N <= 128u * E) many ? k_layer_norm<T, VEC, 64, 2 * S, (MANY + 1) / 2><<<div_up(g4, (MANY + 1) / 2), 256, 0, st>>>(a) : k_layer_norm<T, VEC, 64, 2 * S, 1><<<g4, 256, 0, st>>>(a);
+    // Rows of a wavefront at a time: four where half its lanes have a row's elements and there are rows for every wavefront of the chip, so that as many bytes are in flight
+    // (200 000 x 64 fp32: 39 us one by one, 33 four at a time; 32 768 x 512: 22 either way).  16-bit rows are bound by their conversions instead (65 537 x 128: 18.0 one by one,
+    // 19.0 four at a time).
+    constexpr int MANY = VEC == 1 || sizeof(T) == 2 ? 1 : 4;
+    if (MANY > 1 && a.N <= 32u * E && a.M >= (uint64_t)cu_count() * 64) k_layer_norm<T, VEC, 64, S, MANY><<<div_up(g4, MANY), 256, 0, st>>>(a);
+    else if (a.N <= 64u * E) k_layer_norm<T, VEC, 64, S, 1><<<g4, 256, 0, st>>>(a);
+    else if (a.N <= 128u * E) k_layer_norm<T, VEC, 64, 2 * S, 1><<<g4, 256, 0, st>>>(a);
     else if (a.N <= 256u * E) k_layer_norm<T, VEC, 256, S, 1><<<g1, 256, 0, st>>>(a);
     else if (a.N <= 512u * E) k_layer_norm<T, VEC, 256, 2 * S, 1><<<g1, 256, 0, st>>>(a);
     else if (a.N <= 1024u * E) k_layer_norm<T, VEC, 256, 4 * S, 1><<<g1, 256, 0, st>>>(a);
@@ -433,10 +439,11 @@ template <typename T, int VEC>
 static void ln_backward(const LnArgs &a, uint32_t groups, hipStream_t st) {
     constexpr int E = VEC == 1 ? 8 : VEC, S = E / VEC;
     const uint32_t lds = a.partial ? 2 * a.N * 4 : 0;
-    constexpr int MANY = VEC == 1 ? 1 : 4;             // (as in the forward pass)
-    const bool many = a.M >= (uint64_t)cu_count() * 64;
-    if (a.N <= 64u * E) many ? k_layer_norm_bwd<T, VEC, 64, S, MANY><<<groups, 256, lds, st>>>(a) : k_layer_norm_bwd<T, VEC, 64, S, 1><<<groups, 256, lds, st>>>(a);
-    else if (a.N <= 128u * E) many ? k_layer_norm_bwd<T, VEC, 64, 2 * S, (MANY + 1) / 2><<<groups, 256, lds, st>>>(a) : k_layer_norm_bwd<T, VEC, 64, 2 * S, 1><<<groups, 256, lds, st>>>(a);
+    // (as in the forward pass; 200 000 x 64: fp32 56 us one by one, 48 four at a time, bf16 73 and 65)
+    constexpr int MANY = VEC == 1 ? 1 : 4;
+    if (MANY > 1 && a.N <= 32u * E && a.M >= (uint64_t)cu_count() * 64) k_layer_norm_bwd<T, VEC, 64, S, MANY><<<groups, 256, lds, st>>>(a);
+    else if (a.N <= 64u * E) k_layer_norm_bwd<T, VEC, 64, S, 1><<<groups, 256, lds, st>>>(a);
+    else if (a.N <= 128u * E) k_layer_norm_bwd<T, VEC, 64, 2 * S, 1><<<groups, 256, lds, st>>>(a);
     else if (a.N <= 256u * E) k_layer_norm_bwd<T, VEC, 256, S, 1><<<groups, 256, 0, st>>>(a);
     else if (a.N <= 512u * E) k_layer_norm_bwd<T, VEC, 256, 2 * S, 1><<<groups, 256, 0, st>>>(a);
     else {

@@ -8,6 +8,7 @@
 //
 // Bound by memory: every element is read and written once.  A workgroup takes a few tokens, computes their cosines and sines once into LDS (they are shared by all
 // heads of both tensors: queries and keys go through in ONE launch) and streams the heads in 16-byte vectors.
+// Measured: 16 384 tokens x (16 + 4) heads x 128 bf16: 34 us (168 MB, 4.9 TB/s; one element at a time: 87); 3 x 1 023 x 9 x 40 fp32: 5.4 us (8.8 MB); 8 tokens: 3.6 us, a launch.
 #include "gfpp_common.h"
 
 namespace gfpp {
@@ -175,7 +176,8 @@ GFPP_API int gfpp_rotary(const void *x0, const int64_t *x0_strides, uint32_t hea
     a.D = D;
     a.axes = axes;
     a.sign = backward ? -1.0f : 1.0f;
-    // tokens per workgroup: as many as fill the threads with angles, fewer while the chip is not full
+    // tokens per workgroup: as many as fill the threads with angles (16 384 x 20 heads x 128: four 34 us, one 39), fewer while the chip is not full
+    // (3 069 x 9 heads x 40: two 5.3 us, sixteen 9.3, one 7.0)
     const uint64_t tokens = (uint64_t)B * T;
     uint32_t tw = kRoThreads / a.P;
     tw = tw < 1 ? 1 : (tw > 16 ? 16 : tw);
