@@ -19,7 +19,11 @@ constexpr int wa_bn() { return FEW || (sizeof(T) == 4 && DP == 128) || (sizeof(T
 
 // FEW: a query sees at most 64 keys (wa_few): small tiles, and in the 16-bit modes probabilities as a rounded value and its remainder (window_attn_device.h).
 // HEADS 2: eight wavefronts, four for each of two query heads of a group, share the tiles of keys and values -- half the loads and LDS writes per query.
-// WAVES 1: 32 queries a workgroup instead of 128, for few keys and a grid that would leave CUs empty.
+// WAVES 1: 32 queries a workgroup instead of 128, for few keys and a grid that would leave CUs empty (296 x 4 heads x 16, window 8, fp32: 8.5 us, with 128 queries 13.8).
+// VEC: 16-byte accesses (wa_vectors); one element at a time otherwise (13 000 x 8 heads x 64, window 1 024: 69 and 180 us).
+//
+// Bound by the barrier of every tile and the tiles' way through LDS, then by the matrix pipe.  Measured (bf16): 16 384 x 16 heads on 4 x 128, window 2 049: 313 us (266 GFLOP,
+// 0.85 PFLOP/s); 13 000 x 8 on 2 x 64, window 1 024, 4 sinks: 69 us (26 GFLOP, 0.38 PFLOP/s: at 64 features every 64 products come with an exponential).
 template <typename T, int DP, bool VEC, bool FEW, int HEADS, int WAVES>
 __global__ __launch_bounds__(64 * WAVES * HEADS, WAVES == 1 ? 1 : (sizeof(T) == 2 ? (DP <= 64 && VEC ? (FEW ? 3 : 4) : (VEC || HEADS == 2 ? 2 : 1)) : 1)) void k_window_attn(WaArgs a) {
     constexpr int BN = wa_bn<T, DP, FEW>(), ROWS = 32 * WAVES, NS = DP / 16, NT = DP / 32, NSUB = BN / 32, PK = wa_pitch_row<T, DP>(), PV = wa_pitch_col<T, DP>();

@@ -16,21 +16,23 @@ int wa_arguments(const char *what, WaArgs &a, const int64_t *strides, int n_tens
                  int32_t right, int32_t sinks, int32_t q_start, const int32_t *lengths, float scale, int dtype);
 bool wa_vectors(const WaTensor &t, int D, size_t size);
 
-// (HEADS: as in the forward pass)
-template <typename T, int DP, bool VEC, int HEADS>
-__global__ __launch_bounds__(kWaThreads * HEADS, sizeof(T) == 2 && (VEC || DP <= 64) ? 2 : 1) void k_window_attn_dq(WaArgs a) {
-    constexpr int BN = DP == 128 && (sizeof(T) == 4 || HEADS == 1) ? 32 : 64, NS = DP / 16, NT = DP / 32, PK = wa_pitch_both<T, DP>(), PV = wa_pitch_row<T, DP>();
+// dq of 128 queries of one head, 32 a wavefront, over tiles of keys and values in LDS; s and dout . v both as K Q^T and V dout^T, so that ds is the operand of dq^T += K^T ds^T
+// without leaving its registers.  Measured (bf16): 16 384 x 16 heads on 4 x 128, window 2 049: 425 us (400 GFLOP, 0.94 PFLOP/s; two heads of a group on one workgroup, as in the
+// forward pass: no difference); 13 000 x 8 on 2 x 64, window 1 024, 4 sinks: 84 us (39 GFLOP, 0.47 PFLOP/s).
+template <typename T, int DP, bool VEC>
+__global__ __launch_bounds__(kWaThreads, sizeof(T) == 2 && (VEC || DP <= 64) ? 2 : 1) void k_window_attn_dq(WaArgs a) {
+    constexpr int BN = DP == 128 ? 32 : 64, NS = DP / 16, NT = DP / 32, PK = wa_pitch_both<T, DP>(), PV = wa_pitch_row<T, DP>();
     typedef typename LpTraits<T>::vec vec;
     __shared__ __attribute__((aligned(16))) unsigned char s_k[2][BN * PK], s_v[2][BN * PV];
     const int q_tiles = (a.Tq + kWaRows - 1) / kWaRows;
     // items: sequence, key head, tile of queries, query head of the group -- those that read the same keys side by side
     uint32_t item = wa_item(blockIdx.x, gridDim.x);
-    const int in_group = (int)(item % (a.G / HEADS)) * HEADS + (HEADS == 2 ? __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 8)) : 0);
-    item /= a.G / HEADS;
+    const int in_group = (int)(item % a.G);
+    item /= a.G;
     const int i0 = (int)(item % q_tiles) * kWaRows;
     item /= q_tiles;
     const int hk = (int)(item % a.Hk), hq = hk * a.G + in_group, b = (int)(item / a.Hk);
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6) & 3), c = lane & 31, h = lane >> 5;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)), c = lane & 31, h = lane >> 5;
     const int n = a.lengths ? a.lengths[b] < a.Tk ? a.lengths[b] : a.Tk : a.Tk;
     const int i = i0 + wave * 32 + c, p = a.q_start + i;
     const bool have = i < a.Tq && p < n;                       // (rows behind the sequence: zeros, whatever they hold)
@@ -72,7 +74,7 @@ __global__ __launch_bounds__(kWaThreads * HEADS, sizeof(T) == 2 && (VEC || DP <=
         for (int r = 0; r < 16; ++r) acc[t][r] = 0.0f;
     const T *kb = static_cast<const T *>(a.k.p) + b * a.k.sb + hk * a.k.sh, *vb = static_cast<const T *>(a.v.p) + b * a.v.sb + hk * a.v.sh;
     // two tiles in flight: the one that the next step stores and the one after it (one alone arrives later than the step that it was requested in takes)
-    WaStage<T, DP, BN, VEC, kWaThreads * HEADS> rk[2], rv[2];
+    WaStage<T, DP, BN, VEC, kWaThreads> rk[2], rv[2];
     auto tile_row = [&](int k) { return (k < range.head ? k : range.lo + k - range.head) * BN; };
     // Loads and stores of tiles are unconditional -- past the last tile a load's range is empty, nothing is read --: a load behind a branch may or may not be in flight, and
     // every wait would then be for all of them.
@@ -142,30 +144,34 @@ __global__ __launch_bounds__(kWaThreads * HEADS, sizeof(T) == 2 && (VEC || DP <=
     if (i < a.Tq) wa_store_rows<T, NT, VEC>(acc, a.scale, static_cast<T *>(a.dq.p) + b * a.dq.sb + (int64_t)i * a.dq.st + hq * a.dq.sh, h, a.D);
 }
 
-// dk and dv of 128 (64) keys, the queries in tiles of 32 through LDS.  Two wavefronts for every 32 keys: one makes the probabilities and sums dv, the other takes
-// them a tile later (through LDS, in fp32), makes ds and sums dk.  One wavefront doing both would hold 128 accumulators, 64 registers of K and V and both products:
-// alone on its SIMD, 23 % of the matrix pipe's cycles were used.  Halved, two or more share a SIMD and fill each other's waits; the work is the same (four
-// products per tile, none twice).  Three tiles are held: the one being stored, the one that is read by the first wavefronts and the one that is read by the second.
+// dk and dv of 64 keys, the queries in tiles of 32 through LDS.  Two wavefronts for every 32 keys: one makes the probabilities and sums dv, the other takes
+// them a tile later (through LDS, in fp32), makes ds and sums dk.  One wavefront doing both would hold 128 accumulators, 64 registers of K and V and both products, and
+// be alone on its SIMD.  Halved, two or three share a SIMD and fill each other's waits; the work is the same (four products per tile, none twice).
+// Three tiles are held: the one being stored, the one that is read by the first wavefronts and the one that is read by the second.  AHEAD (16-bit heads of 33 to 64
+// features): the second take their product with dout a tile early and hold it, so that two tiles of dout are enough and three workgroups fit a CU.
 // Work items: first the slices of the tiles with sinks (a.splits each, partial sums), then the other tiles.
-// PAIRS: of wavefronts, 32 keys each: 4, or 2 where 128 keys a workgroup would leave CUs without one (and for the widest fp32 heads, which need the registers).
-constexpr int kWaBq = 32;
-template <typename T, int DP, bool VEC, int PAIRS>
-__global__ __launch_bounds__(PAIRS * 128, PAIRS == 2 && DP == 128 && (sizeof(T) == 4 || !VEC) ? 1 : 2) void k_window_attn_dkv(WaArgs a) {
-    constexpr int KEYS = PAIRS * 32, BQ = kWaBq, NS = DP / 16, NT = DP / 32, PITCH = wa_pitch_both<T, DP>();
+// Bound by the barrier of every tile and the tiles' way through LDS.  Measured (bf16): 16 384 x 16 heads on 4 x 128, window 2 049: 787 us (533 GFLOP, 0.68 PFLOP/s);
+// 13 000 x 8 on 2 x 64, window 1 024, 4 sinks: 155 us (53 GFLOP, 0.34 PFLOP/s).  128 keys a workgroup instead of 64 took within 1.5 % of that at 128 features and 3 to 20 %
+// more at 64 and fewer (16 384 x 16 heads x 64, window 301: dq, dk and dv together 289 us against 237, and 206 with AHEAD).
+constexpr int kWaBq = 32, kWaKeys = 64, kWaPairs = kWaKeys / 32;
+template <typename T, int DP, bool VEC>
+__global__ __launch_bounds__(kWaThreads, DP == 128 && (sizeof(T) == 4 || !VEC) ? 1 : (DP == 64 && sizeof(T) == 2 && VEC ? 3 : 2)) void k_window_attn_dkv(WaArgs a) {
+    constexpr int BQ = kWaBq, NS = DP / 16, NT = DP / 32, PITCH = wa_pitch_both<T, DP>();
+    constexpr bool AHEAD = DP == 64 && sizeof(T) == 2;
     typedef typename LpTraits<T>::vec vec;
     typedef float f4 __attribute__((ext_vector_type(4)));
-    __shared__ __attribute__((aligned(16))) unsigned char s_q[3][BQ * PITCH], s_g[3][BQ * PITCH];
-    __shared__ __attribute__((aligned(16))) float s_p[2][PAIRS][4][64][4];                 // [tile & 1][32 keys][quad of rows][lane][row]
+    __shared__ __attribute__((aligned(16))) unsigned char s_q[3][BQ * PITCH], s_g[AHEAD ? 2 : 3][BQ * PITCH];
+    __shared__ __attribute__((aligned(16))) float s_p[2][kWaPairs][4][64][4];                 // [tile & 1][32 keys][quad of rows][lane][row]
     __shared__ __attribute__((aligned(16))) float s_lse[3][BQ], s_delta[3][BQ];
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)), keys = wave % PAIRS, c = lane & 31, h = lane >> 5;
-    const bool second = wave >= PAIRS;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)), keys = wave % kWaPairs, c = lane & 31, h = lane >> 5;
+    const bool second = wave >= kWaPairs;
     const uint32_t bh = (uint32_t)a.B * a.Hk, sliced = a.sink_tiles * a.splits * bh;
     const bool slice = blockIdx.x < sliced;
     uint32_t item = slice ? blockIdx.x : wa_item(blockIdx.x - sliced, gridDim.x - sliced);
     const uint32_t per_head = slice ? a.sink_tiles * a.splits : (gridDim.x - sliced) / bh, hkb = item / per_head;
     item %= per_head;
     const uint32_t part = slice ? item % a.splits : 0;
-    const int j0 = (int)(slice ? item / a.splits : item + a.sink_tiles) * KEYS;
+    const int j0 = (int)(slice ? item / a.splits : item + a.sink_tiles) * kWaKeys;
     const int hk = (int)(hkb % a.Hk), b = (int)(hkb / a.Hk);
     const int n = a.lengths ? a.lengths[b] < a.Tk ? a.lengths[b] : a.Tk : a.Tk;
     const int jw0 = j0 + keys * 32, jw1 = jw0 + 31, j = jw0 + c;
@@ -180,7 +186,7 @@ __global__ __launch_bounds__(PAIRS * 128, PAIRS == 2 && DP == 128 && (sizeof(T) 
         for (int r = 0; r < 16; ++r) acc[t][r] = 0.0f;
     // query rows [i_lo, i_hi) that can see a key of the tile; rows from `end` on are behind the sequence
     const int end = n - a.q_start < a.Tq ? n - a.q_start : a.Tq;
-    const int jn = j0 + KEYS <= n ? j0 + KEYS - 1 : n - 1;
+    const int jn = j0 + kWaKeys <= n ? j0 + kWaKeys - 1 : n - 1;
     int i_lo = j0 - a.right - a.q_start, i_hi = (j0 < a.sinks ? end : jn + a.left + 1 - a.q_start);
     i_lo = i_lo < 0 ? 0 : i_lo / BQ * BQ;
     i_hi = i_hi < end ? i_hi : end;
@@ -193,7 +199,7 @@ __global__ __launch_bounds__(PAIRS * 128, PAIRS == 2 && DP == 128 && (sizeof(T) 
         tiles = tiles < 0 ? 0 : tiles;
     }
     const int steps = tiles * a.G;
-    WaStage<T, DP, BQ, VEC, PAIRS * 128> rq[2], rg[2];                                 // two tiles in flight (k_window_attn)
+    WaStage<T, DP, BQ, VEC, kWaThreads> rq[2], rg[2];                                 // two tiles in flight (k_window_attn)
     float r_lse[2], r_delta[2];
     int next_tile = 0, next_head = 0, loaded = 0;                                      // of the tile that is loaded next: the heads of a group one after the other
     // (unconditional, as in the forward pass: past the last tile the ranges are empty)
@@ -216,7 +222,7 @@ __global__ __launch_bounds__(PAIRS * 128, PAIRS == 2 && DP == 128 && (sizeof(T) 
     };
     auto store = [&](int buf, int which) {
         rq[which].store(s_q[buf], PITCH);
-        rg[which].store(s_g[buf], PITCH);
+        rg[which].store(s_g[AHEAD ? which : buf], PITCH);
         if (threadIdx.x < BQ) {
             s_lse[buf][threadIdx.x] = r_lse[which];
             s_delta[buf][threadIdx.x] = r_delta[which];
@@ -230,27 +236,29 @@ __global__ __launch_bounds__(PAIRS * 128, PAIRS == 2 && DP == 128 && (sizeof(T) 
     __syncthreads();
     const int row_at = c * PITCH + 8 * h * (int)sizeof(T), col_at = wa_col_offset<T>(lane, PITCH);
     const int from = have ? j - a.right : 0x7fffffff, to = j < a.sinks ? 0x7fffffff : j + a.left;
-    int now = 0, tile = second ? -1 : 0, buf = second ? 2 : 0;                         // buffer of step k; this wavefront's tile and its buffer (one step behind: second)
+    int now = 0, tile = 0, before = 2;                                                 // buffer of tile k, the tile, the buffer of tile k - 1
+    bool seen_before = false;
+    v16f d;                                                                            // second: dout . v of the tile before
     auto step = [&](int k, auto parity) {
         constexpr int odd = decltype(parity)::value;                                   // k & 1; tile k + 1 is in the other registers
         const int next = now == 2 ? 0 : now + 1;
         store(next, odd ^ 1);                                                          // (tile k - 2's: last read a step ago, before the barrier)
         load(odd ^ 1);
         const int p0 = a.q_start + i_lo + tile * BQ, p1 = p0 + BQ - 1;
-        const bool seen = jw0 < n && p1 >= jw0 - a.right && (p0 <= jw1 + a.left || jw0 < a.sinks);
+        const bool seen = k < steps && jw0 < n && p1 >= jw0 - a.right && (p0 <= jw1 + a.left || jw0 < a.sinks);
         if (!second) {
-            if (k < steps && seen) {
+            if (seen) {
                 v16f s;
 #pragma unroll
                 for (int r = 0; r < 16; ++r) s[r] = 0.0f;
                 {
                     WaStream<T, NS> rows;
-                    const auto read = [&](int x) { return wa_row<T>(s_q[buf] + row_at, x); };
+                    const auto read = [&](int x) { return wa_row<T>(s_q[now] + row_at, x); };
                     rows.prime(read);
                     rows.run(read, [&](int x, const vec &y) { s = LpTraits<T>::mfma(y, f[x], s); });
                 }
                 WaStream<T, 2 * NT> cols;
-                const auto read_g = [&](int x) { return wa_col<T, PITCH>(s_g[buf] + col_at, 16 * (x / NT), x % NT); };
+                const auto read_g = [&](int x) { return wa_col<T, PITCH>(s_g[AHEAD ? odd : now] + col_at, 16 * (x / NT), x % NT); };
                 cols.prime(read_g);
                 if (!(jw1 < n && p0 >= jw1 - a.right && (p1 <= jw0 + a.left || jw1 < a.sinks))) {
 #pragma unroll
@@ -261,7 +269,7 @@ __global__ __launch_bounds__(PAIRS * 128, PAIRS == 2 && DP == 128 && (sizeof(T) 
                 }
 #pragma unroll
                 for (int r = 0; r < 16; r += 4) {
-                    const f4 lse = *reinterpret_cast<const f4 *>(&s_lse[buf][2 * r + 4 * h]);
+                    const f4 lse = *reinterpret_cast<const f4 *>(&s_lse[now][2 * r + 4 * h]);
                     f4 pr;
 #pragma unroll
                     for (int e = 0; e < 4; ++e) pr[e] = s[r + e] = __builtin_amdgcn_exp2f(fmaf(s[r + e], a.c, -lse[e]));
@@ -273,34 +281,39 @@ __global__ __launch_bounds__(PAIRS * 128, PAIRS == 2 && DP == 128 && (sizeof(T) 
                     acc[x % NT] = LpTraits<T>::mfma(y, pr, acc[x % NT]);
                 });
             }
-        } else if (k > 0 && seen) {
-            v16f d;
+        } else {
+            auto product = [&](const unsigned char *g) {
 #pragma unroll
-            for (int r = 0; r < 16; ++r) d[r] = 0.0f;
-            {
+                for (int r = 0; r < 16; ++r) d[r] = 0.0f;
                 WaStream<T, NS> rows;
-                const auto read = [&](int x) { return wa_row<T>(s_g[buf] + row_at, x); };
+                const auto read = [&](int x) { return wa_row<T>(g + row_at, x); };
                 rows.prime(read);
                 rows.run(read, [&](int x, const vec &y) { d = LpTraits<T>::mfma(y, f[x], d); });
-            }
-            WaStream<T, 2 * NT> cols;
-            const auto read_q = [&](int x) { return wa_col<T, PITCH>(s_q[buf] + col_at, 16 * (x / NT), x % NT); };
-            cols.prime(read_q);
+            };
+            if (seen_before) {
+                if constexpr (!AHEAD) product(s_g[before]);
+                WaStream<T, 2 * NT> cols;
+                const auto read_q = [&](int x) { return wa_col<T, PITCH>(s_q[before] + col_at, 16 * (x / NT), x % NT); };
+                cols.prime(read_q);
 #pragma unroll
-            for (int r = 0; r < 16; r += 4) {
-                const f4 delta = *reinterpret_cast<const f4 *>(&s_delta[buf][2 * r + 4 * h]), pr = *reinterpret_cast<const f4 *>(s_p[odd ^ 1][keys][r >> 2][lane]);
+                for (int r = 0; r < 16; r += 4) {
+                    const f4 delta = *reinterpret_cast<const f4 *>(&s_delta[before][2 * r + 4 * h]), pr = *reinterpret_cast<const f4 *>(s_p[odd ^ 1][keys][r >> 2][lane]);
 #pragma unroll
-                for (int e = 0; e < 4; ++e) d[r + e] = pr[e] * (d[r + e] - delta[e]);
+                    for (int e = 0; e < 4; ++e) d[r + e] = pr[e] * (d[r + e] - delta[e]);
+                }
+                vec ds;
+                cols.run(read_q, [&](int x, const vec &y) {
+                    if (x % NT == 0) ds = wa_pack<T>(d, x / NT);
+                    acc[x % NT] = LpTraits<T>::mfma(y, ds, acc[x % NT]);
+                });
             }
-            vec ds;
-            cols.run(read_q, [&](int x, const vec &y) {
-                if (x % NT == 0) ds = wa_pack<T>(d, x / NT);
-                acc[x % NT] = LpTraits<T>::mfma(y, ds, acc[x % NT]);
-            });
+            if constexpr (AHEAD)
+                if (seen) product(s_g[odd]);
+            seen_before = seen;
         }
         __syncthreads();
+        before = now;
         now = next;
-        buf = buf == 2 ? 0 : buf + 1;
         if (++tile == tiles) tile = 0;
     };
     for (int k = 0; k <= steps; k += 2) {
@@ -310,7 +323,7 @@ __global__ __launch_bounds__(PAIRS * 128, PAIRS == 2 && DP == 128 && (sizeof(T) 
     if (j >= a.Tk) return;
     const float f_out = second ? a.scale : 1.0f;
     if (slice) {
-        float *out = a.partial + (((((int64_t)(j0 / KEYS) * a.splits + part) * bh + hkb) * 2 + (second ? 0 : 1)) * KEYS + (j - j0)) * a.D;
+        float *out = a.partial + (((((int64_t)(j0 / kWaKeys) * a.splits + part) * bh + hkb) * 2 + (second ? 0 : 1)) * kWaKeys + (j - j0)) * a.D;
         wa_store_rows<float, NT, false>(acc, f_out, out, h, a.D);
     } else {
         const WaTensor &o = second ? a.dk : a.dv;
@@ -318,16 +331,16 @@ __global__ __launch_bounds__(PAIRS * 128, PAIRS == 2 && DP == 128 && (sizeof(T) 
     }
 }
 
-// the slices' sums of the tiles with sinks, added in order
+// the slices' sums of the tiles with sinks, added in order (4 us, a launch)
 template <typename T>
 __global__ __launch_bounds__(kWaThreads) void k_window_attn_join(WaArgs a) {
     const uint32_t bh = (uint32_t)a.B * a.Hk, hkb = blockIdx.y, tile = blockIdx.z;
     const int hk = (int)(hkb % a.Hk), b = (int)(hkb / a.Hk);
-    const int64_t size = 2ll * a.keys * a.D, stride = (int64_t)bh * size;
+    const int64_t size = 2ll * kWaKeys * a.D, stride = (int64_t)bh * size;
     const float *src = a.partial + ((int64_t)tile * a.splits * bh + hkb) * size;
     for (int64_t e = blockIdx.x * kWaThreads + threadIdx.x; e < size; e += (int64_t)gridDim.x * kWaThreads) {
-        const int which = e >= (int64_t)a.keys * a.D, r = (int)(e / a.D) - which * a.keys, d = (int)(e % a.D);
-        const int64_t j = (int64_t)tile * a.keys + r;
+        const int which = e >= (int64_t)kWaKeys * a.D, r = (int)(e / a.D) - which * kWaKeys, d = (int)(e % a.D);
+        const int64_t j = (int64_t)tile * kWaKeys + r;
         if (j >= a.Tk) continue;
         float sum = 0.0f;
         uint32_t s = 0;
@@ -345,31 +358,23 @@ __global__ __launch_bounds__(kWaThreads) void k_window_attn_join(WaArgs a) {
 }
 
 // slices of a tile with sinks: each about the queries that a tile without sinks has, so that no workgroup ends long after the others; at least 256, 64 slices at most
+// (13 000 queries, window 1 024, 4 sinks: 155 us, whole 1 515; a padded batch of 6 x 777, window 251, 3 sinks: 29 us, whole 49)
 static uint32_t wa_splits(const WaArgs &a) {
-    const int64_t ordinary = (int64_t)a.keys + a.left + a.right, each = ordinary > 256 ? ordinary : 256, want = ((int64_t)a.Tq + each - 1) / each;
+    const int64_t ordinary = (int64_t)kWaKeys + a.left + a.right, each = ordinary > 256 ? ordinary : 256, want = ((int64_t)a.Tq + each - 1) / each;
     return (uint32_t)(want < 1 ? 1 : (want > 64 ? 64 : want));
 }
 static uint32_t wa_sink_tiles(const WaArgs &a) {
     // a window that reaches every query from its first key makes the sinks ordinary keys
     if (a.sinks == 0 || (int64_t)a.left + 1 >= (int64_t)a.q_start + a.Tq) return 0;
-    return (uint32_t)((a.sinks + a.keys - 1) / a.keys);
+    return (uint32_t)((a.sinks + kWaKeys - 1) / kWaKeys);
 }
 
 template <typename T, int DP>
 static void wa_backward_launch(const WaArgs &a, bool vec, uint32_t gq, uint32_t gk, hipStream_t st) {
-    if (gq) {
-        bool paired = false;
-        if constexpr (sizeof(T) == 2 && DP == 128) {
-            paired = vec && wa_pair_heads(a, gq);
-            if (paired) k_window_attn_dq<T, DP, true, 2><<<gq / 2, kWaThreads * 2, 0, st>>>(a);
-        }
-        if (!paired) vec ? k_window_attn_dq<T, DP, true, 1><<<gq, kWaThreads, 0, st>>>(a) : k_window_attn_dq<T, DP, false, 1><<<gq, kWaThreads, 0, st>>>(a);
-    }
+    if (gq) vec ? k_window_attn_dq<T, DP, true><<<gq, kWaThreads, 0, st>>>(a) : k_window_attn_dq<T, DP, false><<<gq, kWaThreads, 0, st>>>(a);
     if (!gk) return;
-    if (a.keys == 64) vec ? k_window_attn_dkv<T, DP, true, 2><<<gk, 256, 0, st>>>(a) : k_window_attn_dkv<T, DP, false, 2><<<gk, 256, 0, st>>>(a);
-    if constexpr (sizeof(T) == 2 || DP < 128)
-        if (a.keys == 128) vec ? k_window_attn_dkv<T, DP, true, 4><<<gk, 512, 0, st>>>(a) : k_window_attn_dkv<T, DP, false, 4><<<gk, 512, 0, st>>>(a);
-    if (a.sink_tiles) k_window_attn_join<T><<<dim3(div_up(2 * a.keys * a.D, kWaThreads), (uint32_t)(a.B * a.Hk), a.sink_tiles), kWaThreads, 0, st>>>(a);
+    vec ? k_window_attn_dkv<T, DP, true><<<gk, kWaThreads, 0, st>>>(a) : k_window_attn_dkv<T, DP, false><<<gk, kWaThreads, 0, st>>>(a);
+    if (a.sink_tiles) k_window_attn_join<T><<<dim3(div_up(2 * kWaKeys * a.D, kWaThreads), (uint32_t)(a.B * a.Hk), a.sink_tiles), kWaThreads, 0, st>>>(a);
 }
 template <typename T>
 static void wa_backward(const WaArgs &a, bool vec, uint32_t gq, uint32_t gk, hipStream_t st) {
@@ -390,20 +395,14 @@ using namespace gfpp;
         }                                                              \
     } while (0)
 
-// 128 keys a workgroup, or 64 where there would be fewer than two workgroups for every CU, and for fp32 heads over 64
-static int wa_bwd_keys(const WaArgs &a, int dtype) {
-    const uint64_t groups = (uint64_t)((a.Tk + 127) / 128) * a.B * a.Hk;
-    return groups < 2ull * cu_count() || (dtype == GFPP_F32 && a.D > 64) ? 64 : 128;
-}
-static void wa_bwd_setup(WaArgs &a, int dtype) {
-    a.keys = wa_bwd_keys(a, dtype);
+static void wa_bwd_setup(WaArgs &a) {
     a.sink_tiles = wa_sink_tiles(a);
     a.splits = a.sink_tiles ? wa_splits(a) : 1;
     if (a.splits == 1) a.sink_tiles = 0;                       // whole tiles write their gradients themselves
 }
 
 GFPP_API unsigned long long gfpp_window_attn_backward_scratch_floats(uint32_t B, uint32_t Tq, uint32_t Tk, uint32_t Hq, uint32_t Hk, uint32_t D, int32_t left,
-                                                                     int32_t right, int32_t sinks, int32_t q_start, int dtype) {
+                                                                     int32_t right, int32_t sinks, int32_t q_start, int) {
     if (Hk == 0 || Tq > (1u << 29) || Tk > (1u << 29) || sinks < 0 || left < 0 || right < 0) return 0;
     WaArgs a{};
     a.B = (int)B;
@@ -415,8 +414,8 @@ GFPP_API unsigned long long gfpp_window_attn_backward_scratch_floats(uint32_t B,
     a.right = right < (1 << 29) ? right : 1 << 29;
     a.sinks = sinks < (int)Tk ? sinks : (int)Tk;
     a.q_start = q_start;
-    wa_bwd_setup(a, dtype);
-    return (unsigned long long)B * Hq * Tq + (unsigned long long)a.sink_tiles * a.splits * B * Hk * 2 * a.keys * D;
+    wa_bwd_setup(a);
+    return (unsigned long long)B * Hq * Tq + (unsigned long long)a.sink_tiles * a.splits * B * Hk * 2 * kWaKeys * D;
 }
 
 GFPP_API int gfpp_window_attn_backward(const void *q, const void *k, const void *v, const void *out, const void *out_low, const void *dout, const float *lse, void *dq, void *dk, void *dv,
@@ -438,11 +437,11 @@ GFPP_API int gfpp_window_attn_backward(const void *q, const void *k, const void 
     a.dv.p = dv;
     a.low = wa_two_part(Tk, left, right, sinks, dtype) ? const_cast<void *>(out_low) : nullptr;
     a.lse = const_cast<float *>(lse);
-    wa_bwd_setup(a, dtype);
+    wa_bwd_setup(a);
     a.delta = scratch;
     a.partial = scratch ? scratch + (uint64_t)B * Hq * Tq : nullptr;
     const uint64_t bh = (uint64_t)B * Hk, gq = (uint64_t)div_up(Tq, kWaRows) * Hq * B;
-    const uint64_t gk = ((uint64_t)div_up(Tk, (uint32_t)a.keys) - a.sink_tiles + (uint64_t)a.sink_tiles * a.splits) * bh;
+    const uint64_t gk = ((uint64_t)div_up(Tk, (uint32_t)kWaKeys) - a.sink_tiles + (uint64_t)a.sink_tiles * a.splits) * bh;
     WA_REQUIRE(gq <= 0x7fffffffull && gk <= 0x7fffffffull && (a.sink_tiles == 0 || (bh <= 65535 && a.sink_tiles <= 65535)));
     const size_t size = dtype == GFPP_F32 ? 4 : 2;
     bool vec = (uintptr_t)a.low % 16 == 0;
