@@ -9,7 +9,7 @@
 // fourth tile of 32 slots of its workgroup's stretch, the next tile in flight in registers; the four partial softmaxes meet in LDS.  Few streams: the
 // slots of a stream are split over several workgroups, whose partial results a second launch joins.
 // Probabilities enter the products as a rounded value and its rounded remainder, so that the output carries its own rounding alone.
-// Measured (bf16): 64 streams x 32 heads on 8 x 128, 4 100 slots (1.08 GB): 206 us with the join, 5.2 TB/s, what a copy of 2 GiB reaches; one stream x 8 on 2 x 64, 260 slots:
+// Measured (bf16): 64 streams x 32 heads on 8 x 128, 4 100 slots (1.08 GB): 184 us (5.8 TB/s; a copy of 2 GiB moves 5.2) and 7 for the join; one stream x 8 on 2 x 64, 260 slots:
 // 6.3 us, a launch's latency and four dependent trips to memory.  One element at a time (unaligned rows) takes 1 000 and 23 us.
 // The row of the new token is taken from the arguments by whoever reads that slot, and written by one wavefront: no order between workgroups is needed.
 #include "window_attn_device.h"

@@ -98,6 +98,12 @@ def test_layer_norm_many_rows(dtype, N):
         ref.close(got, want[name], name)
 
 
+@pytest.mark.parametrize("dtype,N", [(torch.float32, 100), (torch.bfloat16, 200), (torch.bfloat16, 8)])
+def test_layer_norm_many_short_rows(dtype, N):
+    """Four rows of a wavefront at a time, the last of them not whole."""
+    test_layer_norm_many_rows(dtype, N)
+
+
 # ---- rotary positions ------------------------------------------------------------------------------------------------------------------------------------
 @pytest.mark.parametrize("dtype", TYPES, ids=IDS)
 @pytest.mark.parametrize("interleaved", [False, True])
@@ -428,6 +434,35 @@ def test_step(B, Hq, Hk, D, slots, sinks, dtype):
             ref.close(out, want, layout)
             same = lambda a, b: torch.equal(a.cpu().nan_to_num(nan=9.0), b.nan_to_num(nan=9.0))  # noqa: E731
             assert same(dk, wk) and same(dv, wv), f"{layout}: one slot of every running stream is written, nothing else"
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS)
+@pytest.mark.parametrize("D,slots,sinks", [(16, 3901, 4), (40, 1570, 0), (64, 767, 1)])
+def test_step_grids_that_fill_the_chip(D, slots, sinks, dtype):
+    """Streams in five, two and one stretches, and key heads turned against the streams: young, full and wrapped ones, the last stretch not whole."""
+    Hk = 8
+    B = torch.cuda.get_device_properties(0).multi_processor_count // 2 // Hk + 1
+    g = gen(slots)
+    q, k, v = rand(g, B, 2 * Hk, D, dtype=dtype), rand(g, B, Hk, D, dtype=dtype), rand(g, B, Hk, D, dtype=dtype)
+    ck, cv = rand(g, B, slots, Hk, D, dtype=dtype), rand(g, B, slots, Hk, D, dtype=dtype)
+    pos = torch.tensor([(7 * slots + 900, slots // 5, -1, slots - 1, slots + 31, 795, 0)[b % 7] for b in range(B)])
+    wk, wv, want = step_reference(q, k, v, ck, cv, pos, sinks)
+    dk, dv = ck.cuda(), cv.cuda()
+    ref.close(window_attention_step(q.cuda(), k.cuda(), v.cuda(), dk, dv, pos.cuda(), sinks), want, "out")
+    assert torch.equal(dk.cpu(), wk) and torch.equal(dv.cpu(), wv)
+
+
+@pytest.mark.parametrize("slots", [640, 1028, 4100])
+def test_step_of_one_stream_in_stretches(slots):
+    g = gen(slots)
+    q, k, v = rand(g, 1, 8, 32, dtype=torch.bfloat16), rand(g, 1, 2, 32, dtype=torch.bfloat16), rand(g, 1, 2, 32, dtype=torch.bfloat16)
+    ck, cv = rand(g, 1, slots, 2, 32, dtype=torch.bfloat16), rand(g, 1, slots, 2, 32, dtype=torch.bfloat16)
+    for n in (slots - 2, slots // 2, 5 * slots + 1):
+        pos = torch.tensor([n])
+        wk, wv, want = step_reference(q, k, v, ck, cv, pos, 4)
+        dk, dv = ck.cuda(), cv.cuda()
+        ref.close(window_attention_step(q.cuda(), k.cuda(), v.cuda(), dk, dv, pos.cuda(), 4), want, n)
+        assert torch.equal(dk.cpu(), wk) and torch.equal(dv.cpu(), wv)
 
 
 # ---- streams, graphs, the run of them together ---------------------------------------------------------------------------------------------------------------
