@@ -11,6 +11,8 @@
 // Measured: 13 000 x 1 024 bf16 with fp32 parameters: forward 12.8 us (53 MB, 4.2 TB/s), backward 21.9 (80 MB, 3.6 TB/s) and 4.0 for the column sums; 65 537 x 204 fp32: forward
 // 24.5 us (107 MB, 4.4 TB/s), backward 28.9 (160 MB, 5.5 TB/s) and 4.0.  Rows that 16-byte vectors do not divide go one element at a time: 24.7 and 36.3, 32.2 and 47.0.
 // One row of 1 024: 2.7 us, a launch.
+#include <algorithm>
+
 #include "gfpp_common.h"
 
 namespace gfpp {
@@ -349,62 +351,70 @@ __global__ __launch_bounds__(256) void k_layer_norm_bwd_long(LnArgs a) {
 }
 template <typename T, int VEC>
 __global__ __launch_bounds__(256) void k_layer_norm_cols_long(LnArgs a) {
-    const uint32_t c = (blockIdx.y * 256 + threadIdx.x) * VEC;
-    if (c >= a.N) return;
-    float dw[VEC], db[VEC];
+    for (uint32_t c = (blockIdx.y * 256 + threadIdx.x) * VEC; c < a.N; c += gridDim.y * 256 * VEC) {
+        float dw[VEC], db[VEC];
 #pragma unroll
-    for (int e = 0; e < VEC; ++e) dw[e] = db[e] = 0.0f;
-    for (uint64_t row = blockIdx.x; row < a.M; row += gridDim.x) {
-        float x[VEC], g[VEC];
-        ln_load<T, VEC>(static_cast<const T *>(a.x) + (int64_t)row * a.xs + c, x);
-        ln_load<T, VEC>(static_cast<const T *>(a.dy) + (int64_t)row * a.dys + c, g);
-        const float mean = a.mean[row], rstd = a.rstd[row];
+        for (int e = 0; e < VEC; ++e) dw[e] = db[e] = 0.0f;
+        for (uint64_t row = blockIdx.x; row < a.M; row += gridDim.x) {
+            float x[VEC], g[VEC];
+            ln_load<T, VEC>(static_cast<const T *>(a.x) + (int64_t)row * a.xs + c, x);
+            ln_load<T, VEC>(static_cast<const T *>(a.dy) + (int64_t)row * a.dys + c, g);
+            const float mean = a.mean[row], rstd = a.rstd[row];
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) {
+                db[e] += g[e];
+                dw[e] = fmaf(g[e], (x[e] - mean) * rstd, dw[e]);
+            }
+        }
+        float *out = a.partial + (uint64_t)blockIdx.x * 2 * a.N + c;
 #pragma unroll
         for (int e = 0; e < VEC; ++e) {
-            db[e] += g[e];
-            dw[e] = fmaf(g[e], (x[e] - mean) * rstd, dw[e]);
+            out[e] = dw[e];
+            out[a.N + e] = db[e];
         }
-    }
-    float *out = a.partial + (uint64_t)blockIdx.x * 2 * a.N + c;
-#pragma unroll
-    for (int e = 0; e < VEC; ++e) {
-        out[e] = dw[e];
-        out[a.N + e] = db[e];
     }
 }
 
-// [P][2][N] partial rows -> dw, db: 32 columns per workgroup, 32 threads down each column, added in a fixed tree
+// [P][2][N] partial rows -> dw, db: 32 columns per workgroup at a time, 32 threads down each column, added in a fixed tree
 template <typename P>
 __global__ __launch_bounds__(1024) void k_layer_norm_cols(const float *__restrict__ partial, uint32_t rows, uint32_t N, P *__restrict__ dw, P *__restrict__ db) {
     __shared__ float s[32][33];
-    const uint32_t c = blockIdx.x * 32 + (threadIdx.x & 31), r0 = threadIdx.x >> 5;
-    float acc = 0.0f;
-    if (c < 2 * N) {
-        uint32_t r = r0;
-        for (; r + 7 * 32 < rows; r += 8 * 32) {               // (eight loads in flight)
-            float v[8];
+    const uint32_t r0 = threadIdx.x >> 5;
+    for (uint32_t c0 = blockIdx.x * 32; c0 < 2 * N; c0 += gridDim.x * 32) {
+        const uint32_t c = c0 + (threadIdx.x & 31);
+        float acc = 0.0f;
+        if (c < 2 * N) {
+            uint32_t r = r0;
+            for (; r + 7 * 32 < rows; r += 8 * 32) {               // (eight loads in flight)
+                float v[8];
 #pragma unroll
-            for (int x = 0; x < 8; ++x) v[x] = partial[(uint64_t)(r + x * 32) * 2 * N + c];
+                for (int x = 0; x < 8; ++x) v[x] = partial[(uint64_t)(r + x * 32) * 2 * N + c];
 #pragma unroll
-            for (int x = 0; x < 8; ++x) acc += v[x];
+                for (int x = 0; x < 8; ++x) acc += v[x];
+            }
+            for (; r < rows; r += 32) acc += partial[(uint64_t)r * 2 * N + c];
         }
-        for (; r < rows; r += 32) acc += partial[(uint64_t)r * 2 * N + c];
-    }
-    s[r0][threadIdx.x & 31] = acc;
-    __syncthreads();
-    // 32 columns x 32 partial sums: the wavefronts read them transposed, 32 lanes per column
-    float v = s[threadIdx.x & 31][threadIdx.x >> 5];
+        s[r0][threadIdx.x & 31] = acc;
+        __syncthreads();
+        // 32 columns x 32 partial sums: the wavefronts read them transposed, 32 lanes per column
+        float v = s[threadIdx.x & 31][threadIdx.x >> 5];
+        __syncthreads();                                           // (read before the next columns' are written)
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor(v, o);
-    const uint32_t col = blockIdx.x * 32 + (threadIdx.x >> 5);
-    if ((threadIdx.x & 31) == 0 && col < 2 * N) {
-        if (col < N) {
-            if (dw) dw[col] = (P)v;
-        } else if (db) {
-            db[col - N] = (P)v;
+        for (int o = 16; o > 0; o >>= 1) v += __shfl_xor(v, o);
+        const uint32_t col = c0 + (threadIdx.x >> 5);
+        if ((threadIdx.x & 31) == 0 && col < 2 * N) {
+            if (col < N) {
+                if (dw) dw[col] = (P)v;
+            } else if (db) {
+                db[col - N] = (P)v;
+            }
         }
     }
 }
+
+// Most workgroups along an axis of columns (wider rows go round again): a grid's axis has to stay below 2^32 threads, and a launch beyond that is not refused -- the count wraps
+// and the columns behind keep what their memory held.
+constexpr uint32_t kLnMostGrid = 32768;
 
 // workgroups of the backward pass = partial rows: four per CU (65 537 x 204 fp32: 28.5 us, two per CU 37.7; 13 000 x 1 024 bf16: 21.9, six per CU 28.9), no more than there
 // are rows to take
@@ -450,7 +460,7 @@ static void ln_backward(const LnArgs &a, uint32_t groups, hipStream_t st) {
     else {
         const uint64_t most = 1u << 22;
         if (a.y) k_layer_norm_bwd_long<T, VEC><<<(uint32_t)(a.M < most ? a.M : most), 256, 0, st>>>(a);
-        if (a.partial) k_layer_norm_cols_long<T, VEC><<<dim3(groups, div_up(a.N, 256 * VEC)), 256, 0, st>>>(a);
+        if (a.partial) k_layer_norm_cols_long<T, VEC><<<dim3(groups, std::min(div_up(a.N, 256 * VEC), kLnMostGrid)), 256, 0, st>>>(a);
     }
 }
 
@@ -513,7 +523,7 @@ GFPP_API int gfpp_layer_norm_backward(const void *dy, int64_t dy_pitch, const vo
     else vec ? ln_backward<__bf16, 8>(a, groups, st) : ln_backward<__bf16, 1>(a, groups, st);
     int rc = check_launch(what);
     if (rc || !cols) return rc;
-    const uint32_t blocks = div_up(2 * N, 32);
+    const uint32_t blocks = std::min(div_up(2 * N, 32), kLnMostGrid);
     if (param_dtype == GFPP_F32) k_layer_norm_cols<float><<<blocks, 1024, 0, st>>>(scratch, groups, N, (float *)dweight, (float *)dbias);
     else if (dtype == GFPP_F16) k_layer_norm_cols<_Float16><<<blocks, 1024, 0, st>>>(scratch, groups, N, (_Float16 *)dweight, (_Float16 *)dbias);
     else k_layer_norm_cols<__bf16><<<blocks, 1024, 0, st>>>(scratch, groups, N, (__bf16 *)dweight, (__bf16 *)dbias);
