@@ -40,6 +40,13 @@ inline int check_launch(const char *what) {
 
 inline uint32_t div_up(uint32_t a, uint32_t b) { return (a + b - 1) / b; }
 
+// Whether the axis of a grid that is a product of counts stays below 2^32 threads.  Beyond that a launch is not refused: the count wraps, and what it leaves out keeps what its
+// memory held.  (Counted in floating point, so that the product itself cannot wrap.)
+template <typename... N>
+inline bool grid_fits(uint32_t threads, N... counts) {
+    return ((1.0 * threads) * ... * (double)counts) < 4294967296.0;
+}
+
 // ---- Morton code: x -> bit 0, y -> bit 1, z -> bit 2 of every 3-bit group ------------------------------------
 __device__ __forceinline__ uint32_t spread3(uint32_t v) {
     v = (v * 0x00010001u) & 0xFF0000FFu;

@@ -184,7 +184,7 @@ GFPP_API int gfpp_rotary(const void *x0, const int64_t *x0_strides, uint32_t hea
     while (tw > 1 && (tokens + tw - 1) / tw < (uint64_t)cu_count() * 4) tw /= 2;
     a.tokens_wg = tw;
     const uint64_t grid = (tokens + tw - 1) / tw;
-    RO_REQUIRE(grid <= 0x7fffffffull);
+    RO_REQUIRE(grid_fits(kRoThreads, grid));
     hipStream_t st = (hipStream_t)stream;
     if (dtype == GFPP_F32) ro_launch<float>(a, vec, interleaved != 0, (uint32_t)grid, st);
     else if (dtype == GFPP_F16) ro_launch<_Float16>(a, vec, interleaved != 0, (uint32_t)grid, st);

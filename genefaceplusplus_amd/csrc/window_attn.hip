@@ -261,13 +261,13 @@ GFPP_API int gfpp_window_attn_forward(const void *q, const void *k, const void *
     a.lse = lse;
     const bool few = wa_few(Tk, left, right, sinks);
     a.low = wa_two_part(Tk, left, right, sinks, dtype) ? out_low : nullptr;
-    const uint64_t grid = (uint64_t)div_up(Tq, kWaRows) * Hq * B;
-    WA_REQUIRE(grid <= 0x7fffffffull);
+    WA_REQUIRE(grid_fits(kWaThreads, div_up(Tq, kWaRows), Hq, B));
+    const uint32_t grid = div_up(Tq, kWaRows) * Hq * B;
     const size_t size = dtype == GFPP_F32 ? 4 : 2;
     const bool vec = wa_vectors(a.q, a.D, size) && wa_vectors(a.k, a.D, size) && wa_vectors(a.v, a.D, size) && wa_vectors(a.o, a.D, size) && (uintptr_t)a.low % 16 == 0;
     hipStream_t st = (hipStream_t)stream;
-    if (dtype == GFPP_F32) wa_forward<float>(a, vec, few, (uint32_t)grid, st);
-    else if (dtype == GFPP_F16) wa_forward<_Float16>(a, vec, few, (uint32_t)grid, st);
-    else wa_forward<__bf16>(a, vec, few, (uint32_t)grid, st);
+    if (dtype == GFPP_F32) wa_forward<float>(a, vec, few, grid, st);
+    else if (dtype == GFPP_F16) wa_forward<_Float16>(a, vec, few, grid, st);
+    else wa_forward<__bf16>(a, vec, few, grid, st);
     return check_launch(what);
 }

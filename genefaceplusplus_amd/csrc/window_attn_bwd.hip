@@ -440,15 +440,16 @@ GFPP_API int gfpp_window_attn_backward(const void *q, const void *k, const void 
     wa_bwd_setup(a);
     a.delta = scratch;
     a.partial = scratch ? scratch + (uint64_t)B * Hq * Tq : nullptr;
-    const uint64_t bh = (uint64_t)B * Hk, gq = (uint64_t)div_up(Tq, kWaRows) * Hq * B;
-    const uint64_t gk = ((uint64_t)div_up(Tk, (uint32_t)kWaKeys) - a.sink_tiles + (uint64_t)a.sink_tiles * a.splits) * bh;
-    WA_REQUIRE(gq <= 0x7fffffffull && gk <= 0x7fffffffull && (a.sink_tiles == 0 || (bh <= 65535 && a.sink_tiles <= 65535)));
+    const uint32_t q_tiles = div_up(Tq, kWaRows), k_tiles = div_up(Tk, (uint32_t)kWaKeys) - a.sink_tiles + a.sink_tiles * a.splits;
+    WA_REQUIRE(grid_fits(kWaThreads, q_tiles, Hq, B) && grid_fits(kWaThreads, k_tiles, Hk, B));
+    const uint32_t bh = B * Hk, gq = q_tiles * Hq * B, gk = k_tiles * bh;
+    WA_REQUIRE(a.sink_tiles == 0 || (bh <= 65535 && a.sink_tiles <= 65535));
     const size_t size = dtype == GFPP_F32 ? 4 : 2;
     bool vec = (uintptr_t)a.low % 16 == 0;
     for (const WaTensor *t : {&a.q, &a.k, &a.v, &a.o, &a.dout, &a.dq, &a.dk, &a.dv}) vec = vec && wa_vectors(*t, a.D, size);
     hipStream_t st = (hipStream_t)stream;
-    if (dtype == GFPP_F32) wa_backward<float>(a, vec, (uint32_t)gq, (uint32_t)gk, st);
-    else if (dtype == GFPP_F16) wa_backward<_Float16>(a, vec, (uint32_t)gq, (uint32_t)gk, st);
-    else wa_backward<__bf16>(a, vec, (uint32_t)gq, (uint32_t)gk, st);
+    if (dtype == GFPP_F32) wa_backward<float>(a, vec, gq, gk, st);
+    else if (dtype == GFPP_F16) wa_backward<_Float16>(a, vec, gq, gk, st);
+    else wa_backward<__bf16>(a, vec, gq, gk, st);
     return check_launch(what);
 }

@@ -16,6 +16,8 @@
 
 namespace gfpp {
 
+constexpr int kWsJoinThreads = 128;                    // a thread per feature
+
 struct WsArgs {
     const void *q, *k, *v;
     void *ck, *cv, *out;
@@ -189,7 +191,7 @@ __global__ __launch_bounds__(kWaThreads, sizeof(T) == 2 ? 2 : 1) void k_window_a
 
 // joins the splits of one (stream, head): a thread per feature
 template <typename T>
-__global__ __launch_bounds__(128) void k_window_attn_step_join(WsArgs a) {
+__global__ __launch_bounds__(kWsJoinThreads) void k_window_attn_step_join(WsArgs a) {
     const int b = (int)(blockIdx.x / a.Hq), hq = (int)(blockIdx.x % a.Hq), d = threadIdx.x;
     if (d >= a.D) return;
     const float *part = a.part + ((int64_t)b * a.Hq + hq) * a.splits * (a.D + 2);
@@ -209,7 +211,7 @@ static void ws_launch(const WsArgs &a, bool vec, uint32_t grid, hipStream_t st) 
     if (a.D <= 32) vec ? k_window_attn_step<T, 32, true><<<grid, kWaThreads, 0, st>>>(a) : k_window_attn_step<T, 32, false><<<grid, kWaThreads, 0, st>>>(a);
     else if (a.D <= 64) vec ? k_window_attn_step<T, 64, true><<<grid, kWaThreads, 0, st>>>(a) : k_window_attn_step<T, 64, false><<<grid, kWaThreads, 0, st>>>(a);
     else vec ? k_window_attn_step<T, 128, true><<<grid, kWaThreads, 0, st>>>(a) : k_window_attn_step<T, 128, false><<<grid, kWaThreads, 0, st>>>(a);
-    if (a.splits > 1) k_window_attn_step_join<T><<<(uint32_t)a.B * a.Hq, 128, 0, st>>>(a);
+    if (a.splits > 1) k_window_attn_step_join<T><<<(uint32_t)a.B * a.Hq, kWsJoinThreads, 0, st>>>(a);
 }
 
 // Stretches that a stream's slots are cut into, us measured with 8 key heads of 128 features, 4 100 slots.
@@ -282,15 +284,15 @@ GFPP_API int gfpp_window_attn_step(const void *q, const void *k, const void *v, 
     a.splits = ws_splits(B, Hq, Hk, slots);
     WS_REQUIRE(a.splits == 1 || scratch);
     a.per_split = (int)(div_up(div_up(slots, a.splits), 32) * 32);
-    const uint64_t grid = (uint64_t)B * Hk * a.chunks * a.splits;
-    WS_REQUIRE(grid <= 0x7fffffffull && (uint64_t)B * Hq <= 0x7fffffffull);
+    WS_REQUIRE(grid_fits(kWaThreads, B, Hk, a.chunks, a.splits) && (a.splits == 1 || grid_fits(kWsJoinThreads, B, Hq)));
+    const uint32_t grid = B * Hk * (uint32_t)a.chunks * a.splits;
     const size_t size = dtype == GFPP_F32 ? 4 : 2;
     uint64_t bits = (uint64_t)(uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)cache_k | (uintptr_t)cache_v | (uint64_t)D * size;
     for (int x = 0; x < 12; ++x) bits |= (uint64_t)s[x] * size;
     const bool vec = bits % 16 == 0;
     hipStream_t st = (hipStream_t)stream;
-    if (dtype == GFPP_F32) ws_launch<float>(a, vec, (uint32_t)grid, st);
-    else if (dtype == GFPP_F16) ws_launch<_Float16>(a, vec, (uint32_t)grid, st);
-    else ws_launch<__bf16>(a, vec, (uint32_t)grid, st);
+    if (dtype == GFPP_F32) ws_launch<float>(a, vec, grid, st);
+    else if (dtype == GFPP_F16) ws_launch<_Float16>(a, vec, grid, st);
+    else ws_launch<__bf16>(a, vec, grid, st);
     return check_launch("gfpp_window_attn_step");
 }

@@ -1,0 +1,40 @@
+"""What the sequence operators promise beside their values, as far as it shows without a GPU: the C entry points check before they launch, the Python ones look at the device last."""
+import ctypes
+
+import pytest
+import torch
+
+from genefaceplusplus_amd import _lib
+
+# ---- the C entry points: every bad call returns its code before a launch (the pointers are never followed) ------------------------------------------------------
+P, EINVAL = 4096, -1
+
+
+def strides(n, value=8):
+    return (ctypes.c_int64 * n)(*[value] * n)
+
+
+def attention_forward(B, Tq, Tk, Hq, Hk, D=8):
+    return _lib.lib().gfpp_window_attn_forward(P, P, P, P, None, None, strides(12), B, Tq, Tk, Hq, Hk, D, 3, 0, 0, 0, None, 1.0, 0, None)
+
+
+def attention_backward(B, Tq, Tk, Hq, Hk, D=8, left=3, sinks=0):
+    return _lib.lib().gfpp_window_attn_backward(P, P, P, P, None, P, P, P, P, P, P, strides(24), B, Tq, Tk, Hq, Hk, D, left, 0, sinks, 0, None, 1.0, 0, None)
+
+
+def step(B, Hq, Hk, slots, D=8, scratch=P):
+    return _lib.lib().gfpp_window_attn_step(P, P, P, P, P, P, 0, P, strides(14), B, Hq, Hk, D, slots, 0, 1.0, 0, scratch, None)
+
+
+def rotary(B, T, heads, D, sections):
+    return _lib.lib().gfpp_rotary(P, strides(3), heads, P, None, None, 0, None, P, 0, 0, P, (ctypes.c_uint32 * len(sections))(*sections), len(sections), B, T, D, 0, 0, 0, None)
+
+
+def test_launches_beyond_a_grid_are_refused():
+    """A launch of 2^32 threads along an axis or more would wrap and leave outputs unwritten: it is an error."""
+    most = 2 ** 24                       # workgroups of 256 threads
+    for call in (lambda: attention_forward(2 ** 20, 8, 8, 16, 1), lambda: attention_forward(1, 2 ** 29, 8, 4, 4), lambda: attention_forward(2 ** 29, 2 ** 29, 1, 2 ** 29, 1),
+                 lambda: attention_backward(2 ** 20, 8, 8, 16, 1), lambda: attention_backward(2, 4, 2 ** 29, 1, 1), lambda: attention_backward(1, 2, 64, most, most),
+                 lambda: rotary(most, 1, 1, 1024, (512,)), lambda: rotary(2 ** 31, 2 ** 31, 1, 2, (1,)),
+                 lambda: step(most, 1, 1, 100), lambda: step(2 ** 20, 16, 16, 100), lambda: step(2 ** 29, 2 ** 29, 2 ** 29, 1), lambda: step(2 ** 19, 64, 1, 1536)):
+        assert call() == EINVAL and b"grid_fits" in _lib.lib().gfpp_last_error()
