@@ -400,6 +400,9 @@ Tensor window_attention_step(const Tensor &q0, const Tensor &k0, const Tensor &v
                    positions.scalar_type() == at::kLong, out.mutable_data_ptr(), strides, (uint32_t)B, (uint32_t)Hq, (uint32_t)Hk, (uint32_t)D, (uint32_t)slots, (uint32_t)sinks, (float)sc,
                    type_code(what, q), static_cast<float *>(mut(scratch)), stream_of(q)),
           "gfpp_window_attn_step");
+    // written in place: whoever has kept them for a backward pass is told (torch raises there)
+    for (const Tensor *t : {&cache_k, &cache_v})
+        if (!t->is_inference()) t->unsafeGetTensorImpl()->bump_version();
     return out;
 }
 

@@ -20,6 +20,31 @@ def rand(seed, *shape, dtype=torch.float32):
     return torch.randn(*shape, generator=torch.Generator().manual_seed(seed)).to(dtype).cuda()
 
 
+# ---- the step and what autograd keeps ------------------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("view", [False, True])
+def test_step_marks_its_caches_as_changed(view):
+    """Keys and values that a backward pass still needs are not changed behind its back: as with any in-place operation of torch, the backward pass raises."""
+    cache = WindowCache(2, 2, 32, window=6, sinks=1, dtype=torch.float32)
+    cache.fill(rand(0, 2, 7, 2, 32), rand(1, 2, 7, 2, 32))
+    q = rand(2, 2, 3, 4, 32).requires_grad_(True)
+    for changed in (cache.k, cache.v):
+        k, v = (cache.k[:, 1:], cache.v[:, 1:]) if view else (cache.k, cache.v)
+        out = window_attention(q, k, v)
+        before = changed._version
+        with torch.no_grad():
+            cache.step(rand(3, 2, 4, 32), rand(4, 2, 2, 32), rand(5, 2, 2, 32))
+        assert changed._version > before
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            out.sum().backward()
+    # nothing in between: the gradient is there
+    window_attention(q, cache.k, cache.v).sum().backward()
+    assert torch.isfinite(q.grad).all()
+    with torch.inference_mode():                              # (tensors without a version)
+        live = WindowCache(2, 2, 32, window=6, sinks=1, dtype=torch.float32)
+        live.step(rand(3, 2, 4, 32), rand(4, 2, 2, 32), rand(5, 2, 2, 32))
+        assert live.positions.tolist() == [1, 1]
+
+
 # ---- sizes at the edges ----------------------------------------------------------------------------------------------------------------------------------------
 def test_layer_norm_of_very_wide_rows():
     """More columns than 2^16 workgroups of the column sums take side by side, more than 2^32 threads of the last launch."""
