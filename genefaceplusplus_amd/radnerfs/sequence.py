@@ -128,7 +128,8 @@ class WindowCache:
         self.positions.copy_(n.view(B))
 
     def step(self, q, k, v, scale=None):
-        """window_attention_step at every stream's next position, which moves on by one."""
+        """window_attention_step at every stream's next position, which moves on by one.  A stream whose position has been set to a negative number rests: its output is
+        zeros, its rows and its position stay until it is given one that is not."""
         out = window_attention_step(q, k, v, self.k, self.v, self.positions, self.sinks, scale)
-        self.positions += 1
+        self.positions += self.positions >= 0
         return out

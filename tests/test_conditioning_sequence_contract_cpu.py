@@ -5,6 +5,7 @@ import pytest
 import torch
 
 from genefaceplusplus_amd import _lib
+from genefaceplusplus_amd.radnerfs import WindowCache, sequence
 
 # ---- the C entry points: every bad call returns its code before a launch (the pointers are never followed) ------------------------------------------------------
 P, EINVAL = 4096, -1
@@ -38,3 +39,17 @@ def test_launches_beyond_a_grid_are_refused():
                  lambda: rotary(most, 1, 1, 1024, (512,)), lambda: rotary(2 ** 31, 2 ** 31, 1, 2, (1,)),
                  lambda: step(most, 1, 1, 100), lambda: step(2 ** 20, 16, 16, 100), lambda: step(2 ** 29, 2 ** 29, 2 ** 29, 1), lambda: step(2 ** 19, 64, 1, 1536)):
         assert call() == EINVAL and b"grid_fits" in _lib.lib().gfpp_last_error()
+
+
+# ---- the Python side ---------------------------------------------------------------------------------------------------------------------------------------
+def test_a_cache_moves_the_running_streams_alone(monkeypatch):
+    """The position of a stream that rests (negative) stays; the step itself is stubbed out here."""
+    monkeypatch.setattr(sequence, "window_attention_step", lambda q, *rest: q)
+    cache = WindowCache(4, 1, 8, 4, 1, dtype=torch.float32, device="cpu")
+    kept = cache.positions
+    cache.positions.copy_(torch.tensor([-1, 5, 0, -2 ** 31]))
+    x = torch.zeros(4, 1, 8)
+    for t in range(1, 4):
+        cache.step(x, x, x)
+        assert cache.positions.tolist() == [-1, 5 + t, t, -2 ** 31] and cache.positions.dtype == torch.int32
+    assert cache.positions is kept

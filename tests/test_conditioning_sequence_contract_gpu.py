@@ -45,6 +45,47 @@ def test_step_marks_its_caches_as_changed(view):
         assert live.positions.tolist() == [1, 1]
 
 
+# ---- streams that rest -----------------------------------------------------------------------------------------------------------------------------------
+def test_parked_streams_stay():
+    """A stream at a negative position: neither its rows nor its position move, however many steps the others take; put back, it goes on where it was."""
+    B, T, Hq, Hk, D, window, sinks = 3, 12, 4, 2, 32, 5, 2
+    q, k, v = rand(0, B, T, Hq, D), rand(1, B, T, Hk, D), rand(2, B, T, Hk, D)
+    parked, free = (WindowCache(B, Hk, D, window, sinks, dtype=torch.float32) for _ in range(2))
+    for t in range(4):
+        parked.step(q[:, t], k[:, t], v[:, t]), free.step(q[:, t], k[:, t], v[:, t])
+    held, rows = parked.positions[1].clone(), parked.k[1].clone()
+    parked.positions[1] = -1
+    for t in range(4, 9):
+        out, want = parked.step(q[:, t], k[:, t], v[:, t]), free.step(q[:, t], k[:, t], v[:, t])
+        assert not out[1].any() and torch.equal(out[::2], want[::2])
+        assert parked.positions.tolist() == [t + 1, -1, t + 1] and torch.equal(parked.k[1], rows)
+    parked.positions[1] = held
+    alone = WindowCache(1, Hk, D, window, sinks, dtype=torch.float32)
+    for t in (0, 1, 2, 3, 9, 10):
+        want = alone.step(q[1:2, t], k[1:2, t], v[1:2, t])
+        if t >= 9:
+            assert torch.equal(parked.step(q[:, t], k[:, t], v[:, t])[1:2], want)
+
+
+def test_parked_streams_stay_in_a_graph():
+    cache = WindowCache(2, 1, 16, 4, 1, dtype=torch.float32)
+    q, k = rand(0, 2, 2, 16), rand(1, 2, 1, 16)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        cache.step(q, k, k)
+    torch.cuda.current_stream().wait_stream(side)
+    cache.positions.copy_(torch.tensor([3, -5]))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        cache.step(q, k, k)
+    rows = cache.k[1].clone()
+    for t in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        assert cache.positions.tolist() == [4 + t, -5] and torch.equal(cache.k[1], rows)
+
+
 # ---- sizes at the edges ----------------------------------------------------------------------------------------------------------------------------------------
 def test_layer_norm_of_very_wide_rows():
     """More columns than 2^16 workgroups of the column sums take side by side, more than 2^32 threads of the last launch."""
