@@ -96,6 +96,12 @@ void same_device(const char *what, const char *name, const Tensor &t, const Tens
 // (the last check of every operator: what else is wrong with a call is told without a GPU too)
 void on_gpu(const char *what, const Tensor &t) { require(t.is_cuda(), what, ": tensors must be on the GPU (no CPU path)"); }
 
+// Derivatives in forward mode: a tensor with a tangent need not ask for a gradient, and no operation is recorded that would carry the tangent on.
+template <typename... T>
+void no_tangents(const char *what, const T &...tensors) {
+    require(!((tensors.defined() && tensors._fw_grad(0).defined()) || ...), what, ": no derivatives in forward mode (an input has a tangent)");
+}
+
 // (an absent tensor reaches an autograd node as an empty optional: it is no input of the node then)
 std::optional<Tensor> given(const Tensor &t) { return t.defined() ? std::optional<Tensor>(t) : std::nullopt; }
 bool wants_grad(const Tensor &t) { return t.defined() && t.requires_grad(); }
@@ -176,6 +182,7 @@ Tensor layer_norm(const Tensor &x, const std::optional<Tensor> &w, const std::op
     require(!weight.defined() || !bias.defined() || weight.scalar_type() == bias.scalar_type(), what, ": weight is ", weight.defined() ? weight.scalar_type() : at::kFloat, ", bias ",
             bias.defined() ? bias.scalar_type() : at::kFloat);
     require(eps >= 0.0, what, ": eps must not be negative, got ", eps);
+    no_tangents(what, x, weight, bias);
     on_gpu(what, x);
     const c10::DeviceGuard guard(x.device());
     if (at::GradMode::is_enabled() && (wants_grad(x) || wants_grad(weight) || wants_grad(bias))) return LayerNormFn::apply(x, given(weight), given(bias), eps);
@@ -249,6 +256,8 @@ variable_list rotary_embed(const variable_list &xs, Tensor positions, Tensor fre
     same_device(what, "positions", positions, first);
     same_device(what, "frequencies", frequencies, first);
     require(!at::GradMode::is_enabled() || !(wants_grad(positions) || wants_grad(frequencies)), what, ": positions and frequencies get no gradient");
+    for (const Tensor &t : xs) no_tangents(what, t);
+    no_tangents(what, positions, frequencies);
     on_gpu(what, first);
     const c10::DeviceGuard guard(first.device());
     positions = positions.contiguous();
@@ -354,6 +363,7 @@ Tensor window_attention(const Tensor &q0, const Tensor &k0, const Tensor &v0, st
                 ": lengths must be an int32 or int64 tensor [", B, "]");
         same_device(what, "lengths", lengths, q0);
     }
+    no_tangents(what, q0, k0, v0);
     on_gpu(what, q0);
     const c10::DeviceGuard guard(q0.device());
     if (lengths.defined()) lengths = lengths.scalar_type() == at::kLong ? lengths.clamp(0, Tk).to(at::kInt) : lengths.contiguous();
@@ -388,6 +398,7 @@ Tensor window_attention_step(const Tensor &q0, const Tensor &k0, const Tensor &v
     require(!at::GradMode::is_enabled() || !(wants_grad(q0) || wants_grad(k0) || wants_grad(v0) || wants_grad(cache_k) || wants_grad(cache_v)), what,
             ": no gradients (call it under torch.no_grad(); window_attention is the differentiable form)");
     const double sc = checked_scale(what, scale, D);
+    no_tangents(what, q0, k0, v0, cache_k, cache_v);
     on_gpu(what, q0);
     const c10::DeviceGuard guard(q0.device());
     const Tensor q = dense_heads(q0), k = dense_heads(k0), v = dense_heads(v0);

@@ -3,9 +3,11 @@ import ctypes
 
 import pytest
 import torch
+import torch.autograd.forward_ad as forward_ad
 
 from genefaceplusplus_amd import _lib
-from genefaceplusplus_amd.radnerfs import WindowCache, sequence
+from genefaceplusplus_amd._lib import GfppError
+from genefaceplusplus_amd.radnerfs import WindowCache, layer_norm, rotary_embed, sequence, window_attention, window_attention_step
 
 # ---- the C entry points: every bad call returns its code before a launch (the pointers are never followed) ------------------------------------------------------
 P, EINVAL = 4096, -1
@@ -53,3 +55,31 @@ def test_a_cache_moves_the_running_streams_alone(monkeypatch):
         cache.step(x, x, x)
         assert cache.positions.tolist() == [-1, 5 + t, t, -2 ** 31] and cache.positions.dtype == torch.int32
     assert cache.positions is kept
+
+
+def sequence_calls():
+    """One call of every operator without fault (but for the device), and the tensors of floating point that it takes, by argument."""
+    z = lambda *shape: torch.zeros(*shape)  # noqa: E731
+    x, q, t = z(3, 8), z(2, 5, 4, 8), z(2, 4, 8)
+    return [(layer_norm, dict(x=x, weight=z(8), bias=z(8)), ("x", "weight", "bias")),
+            (rotary_embed, dict(x=q, positions=z(5, 1), frequencies=z(4).double(), sections=(4,)), ("x", "positions", "frequencies")),
+            (lambda k, **how: rotary_embed((q, k), **how), dict(k=z(2, 5, 1, 8), positions=z(5, 1), frequencies=z(4).double(), sections=(4,)), ("k",)),
+            (window_attention, dict(q=q, k=q, v=q), ("q", "k", "v")),
+            (window_attention_step, dict(q=t, k=t, v=t, cache_k=z(2, 6, 4, 8), cache_v=z(2, 6, 4, 8), positions=torch.zeros(2, dtype=torch.int32)), ("q", "k", "v", "cache_k", "cache_v"))]
+
+
+def test_tangents_are_refused():
+    """A dual tensor does not ask for a gradient: without a check its tangent would be dropped in silence."""
+    for call, args, names in sequence_calls():
+        with pytest.raises(GfppError, match="must be on the GPU"):
+            call(**args)
+        for name in names:
+            with forward_ad.dual_level():
+                dual = forward_ad.make_dual(args[name], torch.ones_like(args[name]))
+                assert not dual.requires_grad
+                with pytest.raises(GfppError, match="forward mode"):
+                    call(**{**args, name: dual})
+                with torch.no_grad(), pytest.raises(GfppError, match="forward mode"):
+                    call(**{**args, name: dual})
+        with pytest.raises(GfppError, match="must be on the GPU"):
+            call(**args)
