@@ -8,8 +8,10 @@
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/utils/pybind.h>
 #include <ATen/ATen.h>
+#include <ATen/TracerMode.h>
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
 #include <c10/core/DeviceGuard.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 
 #include <cmath>
 #include <limits>
@@ -102,6 +104,12 @@ void no_tangents(const char *what, const T &...tensors) {
     require(!((tensors.defined() && tensors._fw_grad(0).defined()) || ...), what, ": no derivatives in forward mode (an input has a tangent)");
 }
 
+// Tracers (torch.jit.trace, make_fx) see the allocation of an output and not the kernel that fills it: what they recorded would return memory as it comes.
+void not_traced(const char *what) {
+    require(!at::tracer::impl::is_dispatch_enabled() && !c10::impl::TorchDispatchModeTLS::get_mode(c10::impl::TorchDispatchModeKey::PROXY).has_value(), what,
+            ": cannot be traced (its kernels are no operations of torch)");
+}
+
 // (an absent tensor reaches an autograd node as an empty optional: it is no input of the node then)
 std::optional<Tensor> given(const Tensor &t) { return t.defined() ? std::optional<Tensor>(t) : std::nullopt; }
 bool wants_grad(const Tensor &t) { return t.defined() && t.requires_grad(); }
@@ -145,6 +153,7 @@ struct LayerNormFn : torch::autograd::Function<LayerNormFn> {
         return y;
     }
     static variable_list backward(AutogradContext *ctx, variable_list grads) {
+        not_traced("layer_norm");
         const auto saved = ctx->get_saved_variables();
         const Tensor &rows = saved[0], &weight = saved[1], &bias = saved[2], &stats = saved[3];
         const Tensor &dy = grads[0];
@@ -183,6 +192,7 @@ Tensor layer_norm(const Tensor &x, const std::optional<Tensor> &w, const std::op
             bias.defined() ? bias.scalar_type() : at::kFloat);
     require(eps >= 0.0, what, ": eps must not be negative, got ", eps);
     no_tangents(what, x, weight, bias);
+    not_traced(what);
     on_gpu(what, x);
     const c10::DeviceGuard guard(x.device());
     if (at::GradMode::is_enabled() && (wants_grad(x) || wants_grad(weight) || wants_grad(bias))) return LayerNormFn::apply(x, given(weight), given(bias), eps);
@@ -221,6 +231,7 @@ struct RotaryFn : torch::autograd::Function<RotaryFn> {
         return rotary_launch(b ? variable_list{a, *b} : variable_list{a}, positions, frequencies, sections, interleaved, false);
     }
     static variable_list backward(AutogradContext *ctx, variable_list grads) {
+        not_traced("rotary_embed");
         const auto saved = ctx->get_saved_variables();
         // the transpose of a turn is the turn by the opposite angle (a tensor that needs no gradient still takes its place in the launch: they come in pairs)
         variable_list out = once(rotary_launch(grads, saved[0], saved[1], ctx->saved_data["sections"].toIntVector(), ctx->saved_data["interleaved"].toBool(), true));
@@ -258,6 +269,7 @@ variable_list rotary_embed(const variable_list &xs, Tensor positions, Tensor fre
     require(!at::GradMode::is_enabled() || !(wants_grad(positions) || wants_grad(frequencies)), what, ": positions and frequencies get no gradient");
     for (const Tensor &t : xs) no_tangents(what, t);
     no_tangents(what, positions, frequencies);
+    not_traced(what);
     on_gpu(what, first);
     const c10::DeviceGuard guard(first.device());
     positions = positions.contiguous();
@@ -303,6 +315,7 @@ struct WindowAttentionFn : torch::autograd::Function<WindowAttentionFn> {
         return out;
     }
     static variable_list backward(AutogradContext *ctx, variable_list grads) {
+        not_traced("window_attention");
         const auto saved = ctx->get_saved_variables();
         const Tensor &q = saved[0], &k = saved[1], &v = saved[2], &out = saved[3], &lse = saved[4], &lengths = saved[5], &low = saved[6];
         const Tensor dout = dense_heads(grads[0]);
@@ -364,6 +377,7 @@ Tensor window_attention(const Tensor &q0, const Tensor &k0, const Tensor &v0, st
         same_device(what, "lengths", lengths, q0);
     }
     no_tangents(what, q0, k0, v0);
+    not_traced(what);
     on_gpu(what, q0);
     const c10::DeviceGuard guard(q0.device());
     if (lengths.defined()) lengths = lengths.scalar_type() == at::kLong ? lengths.clamp(0, Tk).to(at::kInt) : lengths.contiguous();
@@ -399,6 +413,7 @@ Tensor window_attention_step(const Tensor &q0, const Tensor &k0, const Tensor &v
             ": no gradients (call it under torch.no_grad(); window_attention is the differentiable form)");
     const double sc = checked_scale(what, scale, D);
     no_tangents(what, q0, k0, v0, cache_k, cache_v);
+    not_traced(what);
     on_gpu(what, q0);
     const c10::DeviceGuard guard(q0.device());
     const Tensor q = dense_heads(q0), k = dense_heads(k0), v = dense_heads(v0);

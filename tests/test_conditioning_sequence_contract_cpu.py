@@ -4,6 +4,7 @@ import ctypes
 import pytest
 import torch
 import torch.autograd.forward_ad as forward_ad
+from torch.fx.experimental.proxy_tensor import make_fx
 
 from genefaceplusplus_amd import _lib
 from genefaceplusplus_amd._lib import GfppError
@@ -81,5 +82,19 @@ def test_tangents_are_refused():
                     call(**{**args, name: dual})
                 with torch.no_grad(), pytest.raises(GfppError, match="forward mode"):
                     call(**{**args, name: dual})
+        with pytest.raises(GfppError, match="must be on the GPU"):
+            call(**args)
+
+
+def test_tracing_is_refused():
+    """A tracer would record the outputs' allocation alone, and replay that."""
+    for call, args, names in sequence_calls():
+        def of(t):
+            out = call(**{**args, names[0]: t})
+            return out if isinstance(out, torch.Tensor) else out[0]
+        with pytest.raises(GfppError, match="traced"):
+            torch.jit.trace(of, (args[names[0]],), check_trace=False)
+        with pytest.raises(GfppError, match="traced"):
+            make_fx(of)(args[names[0]])
         with pytest.raises(GfppError, match="must be on the GPU"):
             call(**args)

@@ -5,6 +5,7 @@ import math
 import pytest
 import torch
 import torch.autograd.forward_ad as forward_ad
+from torch.fx.experimental.proxy_tensor import make_fx
 
 import sequence_reference as ref
 from genefaceplusplus_amd import _lib
@@ -84,6 +85,28 @@ def test_parked_streams_stay_in_a_graph():
         graph.replay()
         torch.cuda.synchronize()
         assert cache.positions.tolist() == [4 + t, -5] and torch.equal(cache.k[1], rows)
+
+
+# ---- transforms that see no kernel ---------------------------------------------------------------------------------------------------------------------------
+def test_transforms_do_not_pass_unseen():
+    x, w = rand(0, 3, 4, 2, 16), rand(1, 16)
+    with pytest.raises(RuntimeError):
+        torch.func.vmap(lambda t: layer_norm(t, w))(x)
+    with pytest.raises(RuntimeError):
+        torch.func.grad(lambda t: layer_norm(t, w).sum())(x)
+    with pytest.raises(RuntimeError):
+        torch.func.jvp(lambda t: layer_norm(t, w), (x,), (x,))
+    with forward_ad.dual_level(), pytest.raises(GfppError, match="forward mode"):
+        layer_norm(forward_ad.make_dual(x, x), w)
+    with pytest.raises(GfppError, match="traced"):
+        torch.jit.trace(lambda t: layer_norm(t, w), (x,), check_trace=False)
+    for call in (lambda t: layer_norm(t, w), lambda t: window_attention(t, t, t), lambda t: RotaryEncoder(16, (8,))(t, torch.arange(4.0, device="cuda")[:, None])):
+        leaf = x.clone().requires_grad_(True)
+        y = call(leaf)
+        with pytest.raises(RuntimeError, match="traced"):
+            make_fx(lambda g: torch.autograd.grad(y, leaf, g, retain_graph=True))(x)
+        assert torch.isfinite(torch.autograd.grad(y, leaf, x)[0]).all()
+    assert not torch.isnan(layer_norm(x, w)).any()
 
 
 # ---- sizes at the edges ----------------------------------------------------------------------------------------------------------------------------------------
