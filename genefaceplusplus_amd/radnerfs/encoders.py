@@ -304,12 +304,22 @@ class RotaryEncoder(nn.Module):
         self.input_dim, self.output_dim = len(self.sections), dim
         self.theta, self.interleaved, self.joint = float(theta), bool(interleaved), bool(joint)
         parts = [P] if self.joint else self.sections
-        self._frequencies = torch.cat([self.theta ** (-torch.arange(n, dtype=torch.float64) / max(n, 1)) for n in parts])
+        with torch.inference_mode(False):               # (what inference_mode makes cannot be kept for a backward pass later)
+            self._frequencies = torch.cat([self.theta ** (-torch.arange(n, dtype=torch.float64, device="cpu") / max(n, 1)) for n in parts])
         self._on = {}                   # (no buffer: module.half() and the like would round it)
+
+    def _apply(self, fn, recurse=True):
+        """Module.to and its like: the frequencies go along to the device, in their own type."""
+        super()._apply(fn, recurse)
+        self.frequencies(fn(torch.empty(1, device="cpu")).device)
+        return self
 
     def frequencies(self, device):
         if device not in self._on:
-            self._on[device] = self._frequencies.to(device)
+            if device.type == "cuda" and torch.cuda.is_current_stream_capturing():
+                raise GfppError(f"RotaryEncoder: its frequencies are not on {device} yet and cannot be copied while a graph is captured: move the module there (.to) before")
+            with torch.inference_mode(False):
+                self._on[device] = self._frequencies.to(device)
         return self._on[device]
 
     def forward(self, x, positions):

@@ -8,7 +8,7 @@ from torch.fx.experimental.proxy_tensor import make_fx
 
 from genefaceplusplus_amd import _lib
 from genefaceplusplus_amd._lib import GfppError
-from genefaceplusplus_amd.radnerfs import WindowCache, layer_norm, rotary_embed, sequence, window_attention, window_attention_step
+from genefaceplusplus_amd.radnerfs import RotaryEncoder, WindowCache, layer_norm, rotary_embed, sequence, window_attention, window_attention_step
 
 # ---- the C entry points: every bad call returns its code before a launch (the pointers are never followed) ------------------------------------------------------
 P, EINVAL = 4096, -1
@@ -98,3 +98,23 @@ def test_tracing_is_refused():
             make_fx(of)(args[names[0]])
         with pytest.raises(GfppError, match="must be on the GPU"):
             call(**args)
+
+
+def test_encoder_keeps_ordinary_frequencies(monkeypatch):
+    """Whatever mode the encoder is made or first called in, its frequencies can be kept for a backward pass; a move takes them along, a change of type leaves them as they are."""
+    meta = torch.device("meta")
+    with torch.inference_mode():
+        encoder = RotaryEncoder(16, (3, 5))
+        encoder.frequencies(meta)
+    for device in (meta, torch.device("cpu")):
+        kept = encoder.frequencies(device)
+        assert not kept.is_inference() and kept.dtype == torch.float64 and kept.shape == (8,) and kept.device == device
+        assert encoder.frequencies(device) is kept
+    with torch.device("meta"):
+        assert torch.equal(RotaryEncoder(16, (3, 5)).frequencies(torch.device("cpu")), encoder.frequencies(torch.device("cpu")))
+    moved = RotaryEncoder(16, (8,)).to("meta").half()
+    assert moved._on[meta].dtype == torch.float64
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    with pytest.raises(GfppError, match="captured"):
+        RotaryEncoder(16, (8,)).frequencies(torch.device("cuda", 0))
+    assert moved.frequencies(meta) is moved._on[meta]

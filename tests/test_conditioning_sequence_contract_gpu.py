@@ -109,6 +109,39 @@ def test_transforms_do_not_pass_unseen():
     assert not torch.isnan(layer_norm(x, w)).any()
 
 
+# ---- the rotary encoder's frequencies ------------------------------------------------------------------------------------------------------------------------
+def test_encoder_serves_first_and_trains_later():
+    """A first call under inference_mode leaves nothing that a later training pass cannot use."""
+    pos = torch.arange(5).cuda()[:, None]
+    x = rand(0, 2, 5, 3, 16)
+    served, fresh = RotaryEncoder(16, (8,)), RotaryEncoder(16, (8,))
+    with torch.inference_mode():
+        served(x, pos)
+    leaf = x.clone().requires_grad_(True)
+    y = served(leaf, pos)
+    assert torch.equal(y, fresh(x, pos))
+    (dx,) = torch.autograd.grad(y, leaf, x)
+    ref.close(dx, ref.rotary(x.cpu(), pos.cpu(), 10000.0 ** (-torch.arange(8, dtype=torch.float64) / 8), (8,), backward=True), "dx")
+
+
+def test_encoder_moved_to_the_gpu_can_be_captured():
+    """Module.to / .cuda() brings the frequencies along (unrounded by .half()), so that the first call may be a captured one; without it capture is refused before it is broken."""
+    pos = torch.arange(6).cuda()[:, None]
+    x = rand(0, 1, 6, 2, 32, dtype=torch.float16)
+    want = RotaryEncoder(32, (16,))(x, pos)
+    moved = RotaryEncoder(32, (16,)).cuda().half()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = moved(x, pos)
+        with pytest.raises(GfppError, match="captur"):
+            RotaryEncoder(32, (16,))(x, pos)
+    for _ in range(3):
+        y.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(y, want)
+
+
 # ---- sizes at the edges ----------------------------------------------------------------------------------------------------------------------------------------
 def test_layer_norm_of_very_wide_rows():
     """More columns than 2^16 workgroups of the column sums take side by side, more than 2^32 threads of the last launch."""
