@@ -13,6 +13,8 @@
 #include <c10/core/DeviceGuard.h>
 #include <c10/core/impl/TorchDispatchModeTLS.h>
 
+#include <algorithm>
+#include <array>
 #include <cmath>
 #include <limits>
 #include <optional>
@@ -387,6 +389,50 @@ Tensor window_attention(const Tensor &q0, const Tensor &k0, const Tensor &v0, st
 }
 
 // ---- the step over a rolling cache ---------------------------------------------------------------------------------------------------------------------------------
+// Whether all elements of some axes (size, stride) lie apart: sorted by stride, every axis steps over what the ones before it span.
+using Axes = std::array<std::pair<int64_t, int64_t>, 5>;
+bool axes_apart(Axes axes) {
+    std::sort(axes.begin(), axes.end(), [](const auto &a, const auto &b) { return a.second < b.second; });
+    int64_t span = 1;
+    for (const auto &[size, stride] : axes) {
+        if (size <= 1) continue;
+        if (stride < span) return false;
+        span += (size - 1) * stride;
+    }
+    return true;
+}
+Axes axes_of(const Tensor &t) {
+    Axes axes{};
+    for (int64_t i = 0; i < 4; ++i) axes[i] = {t.size(i), t.stride(i)};
+    axes[4] = {1, 0};
+    return axes;
+}
+// Caches are written in place, each slot by whoever has it: two slots in one memory, within a cache or between the two, would be a race.
+bool caches_apart(const Tensor &a, const Tensor &b) {
+    if (a.numel() == 0) return true;
+    Axes axes = axes_of(a);
+    const Axes other = axes_of(b);
+    if (!axes_apart(axes) || !axes_apart(other)) return false;
+    const auto bytes = [](const Tensor &t) {
+        int64_t span = 1;
+        for (int64_t i = 0; i < t.dim(); ++i) span += (t.size(i) - 1) * t.stride(i);
+        return span * (int64_t)t.element_size();
+    };
+    const int64_t apart = (int64_t)((intptr_t)b.const_data_ptr() - (intptr_t)a.const_data_ptr()), size = (int64_t)a.element_size();
+    if (apart >= bytes(a) || -apart >= bytes(b)) return true;
+    // One inside the other's reach.  Blocks of keys and of values in turn along an axis, each block as it likes:
+    for (int64_t i = 0; i < 4; ++i) {
+        if (axes[i].first <= 1 || axes[i].second != other[i].second) continue;
+        const int64_t period = axes[i].second * size, rest = (axes[i].first - 1) * period, from = (apart % period + period) % period;
+        if (from >= bytes(a) - rest && period - from >= bytes(b) - rest) return true;
+    }
+    // ... or side by side at any axis with the same strides, which is one more axis of two
+    for (int64_t i = 0; i < 4; ++i)
+        if (axes[i].first > 1 && axes[i].second != other[i].second) return false;
+    axes[4] = {2, std::abs(apart) / size};
+    return apart % size == 0 && axes_apart(axes);
+}
+
 Tensor window_attention_step(const Tensor &q0, const Tensor &k0, const Tensor &v0, const Tensor &cache_k, const Tensor &cache_v, const Tensor &positions, int64_t sinks,
                              std::optional<double> scale) {
     const char *what = "window_attention_step";
@@ -415,6 +461,7 @@ Tensor window_attention_step(const Tensor &q0, const Tensor &k0, const Tensor &v
     no_tangents(what, q0, k0, v0, cache_k, cache_v);
     not_traced(what);
     on_gpu(what, q0);
+    require(caches_apart(cache_k, cache_v), what, ": slots of cache_k and cache_v lie in one memory (strides ", cache_k.strides(), ", ", cache_v.strides(), "): they are written in place");
     const c10::DeviceGuard guard(q0.device());
     const Tensor q = dense_heads(q0), k = dense_heads(k0), v = dense_heads(v0);
     const Tensor out = at::empty(q.sizes(), q.options());

@@ -87,6 +87,34 @@ def test_parked_streams_stay_in_a_graph():
         assert cache.positions.tolist() == [4 + t, -5] and torch.equal(cache.k[1], rows)
 
 
+# ---- memory ------------------------------------------------------------------------------------------------------------------------------------------------
+def test_caches_of_one_memory_are_refused():
+    """Slots that lie in one another, within a cache or between the two, would be written twice; halves of one allocation are apart."""
+    B, slots, Hk, D = 2, 6, 2, 16
+    q, k = rand(0, B, 4, D), rand(1, B, Hk, D)
+    pos = torch.tensor([3, 9]).cuda()
+    room = torch.zeros(4096, device="cuda")
+    dense = (slots * Hk * D, Hk * D, D, 1)
+    at = lambda offset, strides=dense: torch.as_strided(room, (B, slots, Hk, D), strides, offset)  # noqa: E731
+    for ck, cv in ((at(0), at(0)), (at(0), at(D)), (at(0), at(dense[0])), (at(D // 2), at(0)), (at(0, (slots * Hk * D, Hk * D, D - 4, 1)), at(2048)), (at(0), at(1024, (64, Hk * D, D, 1))),
+                   (at(0), at(dense[0] // 2, (slots * Hk * D, D, slots * D, 1)))):
+        with pytest.raises(GfppError, match="one memory"):
+            window_attention_step(q, k, k, ck, cv, pos)
+    assert not room.any()
+    want = window_attention_step(q, k, k, torch.zeros(B, slots, Hk, D, device="cuda"), torch.zeros(B, slots, Hk, D, device="cuda"), pos)
+    tokens = torch.zeros(B, slots, 2, Hk, D, device="cuda")
+    heads = torch.zeros(B, slots, Hk, 2, D, device="cuda")
+    streams = torch.zeros(B, 2, slots, Hk, D, device="cuda")
+    whole = torch.zeros(2, B, slots, Hk, D, device="cuda")
+    swapped = torch.zeros(2, B, Hk, slots, D, device="cuda").transpose(2, 3)
+    blocks = torch.zeros(B, 2, slots * Hk * D, device="cuda")
+    for ck, cv in ((tokens[:, :, 0], tokens[:, :, 1]), (tokens[:, :, 1], tokens[:, :, 0]), (heads[..., 0, :], heads[..., 1, :]), (streams[:, 0], streams[:, 1]), (whole[0], whole[1]),
+                   (swapped[0], swapped[1]), (blocks[:, 0].view(B, Hk, slots, D).transpose(1, 2), blocks[:, 1].view(B, slots, Hk, D)),
+                   (blocks[:, 1].view(B, slots, Hk, D), blocks[:, 0].view(B, Hk, slots, D).transpose(1, 2))):
+        ck.zero_(), cv.zero_()
+        assert torch.equal(window_attention_step(q, k, k, ck, cv, pos), want)
+
+
 # ---- transforms that see no kernel ---------------------------------------------------------------------------------------------------------------------------
 def test_transforms_do_not_pass_unseen():
     x, w = rand(0, 3, 4, 2, 16), rand(1, 16)
