@@ -110,8 +110,10 @@ class WindowCache:
             raise GfppError(f"WindowCache.fill: k, v must be [{self.k.shape[0]}, T, {self.k.shape[2]}, {self.k.shape[3]}], got {tuple(k.shape)}, {tuple(v.shape)}")
         if k.dtype != self.k.dtype or v.dtype != self.k.dtype:
             raise GfppError(f"WindowCache.fill: k, v must be {self.k.dtype}, got {k.dtype}, {v.dtype}")
-        if lengths is not None and tuple(lengths.shape) != (B,):
-            raise GfppError(f"WindowCache.fill: lengths must be [{B}], got {tuple(lengths.shape)}")
+        if k.device != self.k.device or v.device != self.k.device:
+            raise GfppError(f"WindowCache.fill: k, v must be on {self.k.device}, got {k.device}, {v.device}")
+        if lengths is not None and (tuple(lengths.shape) != (B,) or lengths.dtype not in (torch.int32, torch.int64) or lengths.device != self.k.device):
+            raise GfppError(f"WindowCache.fill: lengths must be an int32 or int64 tensor [{B}] on {self.k.device}, got {lengths.dtype} {tuple(lengths.shape)} on {lengths.device}")
         n = torch.full((B, 1), T, device=k.device) if lengths is None else lengths.to(torch.int64).clamp(0, T).view(B, 1)
         slot = torch.arange(self.sinks + self.window, device=k.device).view(1, -1)
         # the newest token of every ring slot: the last one before n whose distance from the first ring token leaves the slot's remainder

@@ -58,6 +58,21 @@ def test_a_cache_moves_the_running_streams_alone(monkeypatch):
     assert cache.positions is kept
 
 
+def test_fill_moves_and_casts_nothing():
+    """Keys, values or lengths on another device, lengths that are no whole numbers."""
+    x, here = torch.zeros(2, 3, 1, 8), WindowCache(2, 1, 8, 4, 1, dtype=torch.float32, device="cpu")
+    away = WindowCache(2, 1, 8, 4, 1, dtype=torch.float32, device="meta")
+    for cache, k, v in ((away, x, x), (here, x, x.to("meta")), (here, x.to("meta"), x)):
+        with pytest.raises(GfppError, match="k, v must be on"):
+            cache.fill(k, v)
+    for lengths in (torch.tensor([1.5, 2.0]), torch.tensor([True, False]), torch.tensor([1, 2], device="meta"), torch.tensor([1, 2], dtype=torch.int16)):
+        with pytest.raises(GfppError, match="lengths must be"):
+            here.fill(x, x, lengths)
+    for lengths in (torch.tensor([1, 9]), torch.tensor([1, 3], dtype=torch.int32)):
+        here.fill(x, x, lengths)
+        assert here.positions.tolist() == [1, 3]
+
+
 def sequence_calls():
     """One call of every operator without fault (but for the device), and the tensors of floating point that it takes, by argument."""
     z = lambda *shape: torch.zeros(*shape)  # noqa: E731
