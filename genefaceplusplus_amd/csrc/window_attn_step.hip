@@ -50,7 +50,7 @@ __global__ __launch_bounds__(kWaThreads, sizeof(T) == 2 ? 2 : 1) void k_window_a
     const int64_t n = a.pos64 ? static_cast<const int64_t *>(a.pos)[b] : (int64_t)static_cast<const int32_t *>(a.pos)[b];
     const int window = a.slots - a.sinks;
     const int at = n < 0 ? -1 : (int)(n < a.sinks ? n : a.sinks + (n - a.sinks) % window);
-    const int filled = n < 0 ? 0 : (int)(n + 1 < a.slots ? n + 1 : a.slots);
+    const int filled = n < 0 ? 0 : (int)(n < a.slots - 1 ? n + 1 : a.slots);
     const int g0 = chunk * 32, heads = a.G - g0 < 32 ? a.G - g0 : 32, hq0 = hk * a.G + g0;
     const T *kb = static_cast<const T *>(a.ck) + b * a.ckb + hk * a.ckh, *vb = static_cast<const T *>(a.cv) + b * a.cvb + hk * a.cvh;
     const T *kn = static_cast<const T *>(a.k) + b * a.kb + hk * a.kh, *vn = static_cast<const T *>(a.v) + b * a.vb + hk * a.vh;

@@ -87,6 +87,22 @@ def test_parked_streams_stay_in_a_graph():
         assert cache.positions.tolist() == [4 + t, -5] and torch.equal(cache.k[1], rows)
 
 
+@pytest.mark.parametrize("sinks", [0, 2])
+def test_step_at_the_last_position(sinks):
+    """The largest position that 64 bits hold: a wrapped stream like any other."""
+    slots, last = 7, 2 ** 63 - 1
+    window = slots - sinks
+    near = sinks + (last - sinks) % window + 3 * window        # the same slot, a smaller number
+    q, k, v = rand(0, 1, 2, 16), rand(1, 1, 1, 16), rand(2, 1, 1, 16)
+    outs = []
+    for n in (near, last, last - window):
+        ck, cv = rand(3, 1, slots, 1, 16), rand(4, 1, slots, 1, 16)
+        outs.append((window_attention_step(q, k, v, ck, cv, torch.tensor([n]).cuda(), sinks), ck, cv))
+    for got in outs[1:]:
+        assert all(torch.equal(a, b) for a, b in zip(got, outs[0]))
+    assert outs[0][0].any()
+
+
 # ---- memory ------------------------------------------------------------------------------------------------------------------------------------------------
 def test_caches_of_one_memory_are_refused():
     """Slots that lie in one another, within a cache or between the two, would be written twice; halves of one allocation are apart."""
