@@ -357,11 +357,15 @@ __global__ __launch_bounds__(kWaThreads) void k_window_attn_join(WaArgs a) {
     }
 }
 
-// slices of a tile with sinks: each about the queries that a tile without sinks has, so that no workgroup ends long after the others; at least 256, 64 slices at most
-// (13 000 queries, window 1 024, 4 sinks: 155 us, whole 1 515; a padded batch of 6 x 777, window 251, 3 sinks: 29 us, whole 49)
+// Slices of a tile with sinks: each about the queries that a tile without sinks has, so that no workgroup ends long after the others; at least 256, 64 slices at most
+// (13 000 queries, window 1 024, 4 sinks: 155 us, whole 1 515; a padded batch of 6 x 777, window 251, 3 sinks: 29 us, whole 49).  All tiles' slices together: 4 096 at most, five
+// times what the chip holds at once, so that their partial sums end at 256 MB (128 features) however many sinks and heads there are (whole backward pass, bf16: 13 000 x 8 heads x 128, window 129, 1 000
+// sinks 506 us, without that end 597; 64 x 4 096 x 8 x 64, window 128, 4 sinks 1 350 and 1 417).
+constexpr uint32_t kWaMostSlices = 4096;
 static uint32_t wa_splits(const WaArgs &a) {
     const int64_t ordinary = (int64_t)kWaKeys + a.left + a.right, each = ordinary > 256 ? ordinary : 256, want = ((int64_t)a.Tq + each - 1) / each;
-    return (uint32_t)(want < 1 ? 1 : (want > 64 ? 64 : want));
+    const uint64_t tiles = (uint64_t)a.sink_tiles * a.B * a.Hk, room = kWaMostSlices / (tiles ? tiles : 1), most = room < 64 ? room : 64;
+    return (uint32_t)(want < 1 || most < 1 ? 1 : ((uint64_t)want > most ? most : want));
 }
 static uint32_t wa_sink_tiles(const WaArgs &a) {
     // a window that reaches every query from its first key makes the sinks ordinary keys
@@ -443,7 +447,6 @@ GFPP_API int gfpp_window_attn_backward(const void *q, const void *k, const void 
     const uint32_t q_tiles = div_up(Tq, kWaRows), k_tiles = div_up(Tk, (uint32_t)kWaKeys) - a.sink_tiles + a.sink_tiles * a.splits;
     WA_REQUIRE(grid_fits(kWaThreads, q_tiles, Hq, B) && grid_fits(kWaThreads, k_tiles, Hk, B));
     const uint32_t bh = B * Hk, gq = q_tiles * Hq * B, gk = k_tiles * bh;
-    WA_REQUIRE(a.sink_tiles == 0 || (bh <= 65535 && a.sink_tiles <= 65535));
     const size_t size = dtype == GFPP_F32 ? 4 : 2;
     bool vec = (uintptr_t)a.low % 16 == 0;
     for (const WaTensor *t : {&a.q, &a.k, &a.v, &a.o, &a.dout, &a.dq, &a.dk, &a.dv}) vec = vec && wa_vectors(*t, a.D, size);

@@ -44,6 +44,17 @@ def test_launches_beyond_a_grid_are_refused():
         assert call() == EINVAL and b"grid_fits" in _lib.lib().gfpp_last_error()
 
 
+def test_scratch_of_the_backward_pass_is_bounded():
+    """Beside one float per query and head, the sinks' partial sums: 4 096 slices of 64 keys' dk and dv at most, however many sinks, heads and queries there are."""
+    floats = _lib.lib().gfpp_window_attn_backward_scratch_floats
+    for B, T, H, D, left, sinks in ((1, 13000, 8, 128, 128, 1000), (1, 500000, 8, 128, 64, 400000), (1, 500000, 1, 128, 0, 500000), (64, 4096, 8, 64, 127, 4), (1, 300, 65540, 2, 40, 3),
+                                    (2000, 1000, 32, 128, 10, 1), (1, 100000, 1, 64, 100, 64)):
+        partial = floats(B, T, T, H, H, D, left, 0, sinks, 0, 0) - B * H * T
+        assert 0 <= partial <= 4096 * 2 * 64 * D, (B, T, H, partial)
+        tiles = -(-sinks // 64) * B * H
+        assert partial % (tiles * 2 * 64 * D) == 0 and (partial > 0) == (tiles <= 2048)
+
+
 # ---- the Python side ---------------------------------------------------------------------------------------------------------------------------------------
 def test_a_cache_moves_the_running_streams_alone(monkeypatch):
     """The position of a stream that rests (negative) stays; the step itself is stubbed out here."""

@@ -187,6 +187,36 @@ def test_encoder_moved_to_the_gpu_can_be_captured():
 
 
 # ---- sizes at the edges ----------------------------------------------------------------------------------------------------------------------------------------
+def test_backward_of_very_many_heads_with_sinks():
+    """More (sequence, key head) pairs than a grid's second axis holds, long enough for the sinks' tile to be taken in slices: every head has the same data and the same gradients."""
+    T, H, D = 300, 65540, 2
+    q, k, v, dout = (rand(s, 1, T, 1, D) for s in range(4))
+    how = dict(left=40, right=0, sinks=3)
+    want = ref.attention(*(t.cpu() for t in (q, k, v, dout)), **how)
+    leaves = [t.expand(1, T, H, D).detach().requires_grad_(True) for t in (q, k, v)]
+    out = window_attention(*leaves, **how)
+    for name, got in zip(("out", "dq", "dk", "dv"), (out, *torch.autograd.grad(out, leaves, dout.expand(1, T, H, D)))):
+        assert torch.equal(got, got[:, :, :1].expand_as(got)), name
+        ref.close(got[:, :, :1], want[name], name)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+def test_backward_of_many_sinks(dtype):
+    """Many tiles of sinks of many heads: fewer slices than queries would make, so that their partial sums stay bounded; the same bits every time."""
+    B, T, H, D, lengths = 2, 1100, 64, 16, (1100, 801)
+    q, k, v, dout = (rand(s, B, T, H, D, dtype=dtype) for s in range(4))
+    how = dict(left=20, right=3, sinks=1000)
+    want = ref.attention(q, k, v, dout, lengths=lengths, **how)
+    runs = []
+    for _ in range(2):
+        leaves = [t.detach().requires_grad_(True) for t in (q, k, v)]
+        out = window_attention(*leaves, lengths=torch.tensor(lengths).cuda(), **how)
+        runs.append((out, *torch.autograd.grad(out, leaves, dout)))
+    for name, got, again in zip(("out", "dq", "dk", "dv"), *runs):
+        ref.close(got, want[name], name)
+        assert torch.equal(got, again), name
+
+
 def test_layer_norm_of_very_wide_rows():
     """More columns than 2^16 workgroups of the column sums take side by side, more than 2^32 threads of the last launch."""
     N = 2 ** 26 + 35
