@@ -459,7 +459,7 @@ static void ln_backward(const LnArgs &a, uint32_t groups, hipStream_t st) {
     else if (a.N <= 512u * E) k_layer_norm_bwd<T, VEC, 256, 2 * S, 1><<<groups, 256, 0, st>>>(a);
     else {
         const uint64_t most = 1u << 22;
-        if (a.y) k_layer_norm_bwd_long<T, VEC><<<(uint32_t)(a.M < most ? a.M : most), 256, 0, st>>>(a);
+        if (a.y && a.M) k_layer_norm_bwd_long<T, VEC><<<(uint32_t)(a.M < most ? a.M : most), 256, 0, st>>>(a);
         if (a.partial) k_layer_norm_cols_long<T, VEC><<<dim3(groups, std::min(div_up(a.N, 256 * VEC), kLnMostGrid)), 256, 0, st>>>(a);
     }
 }

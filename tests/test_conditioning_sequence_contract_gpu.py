@@ -229,3 +229,19 @@ def test_layer_norm_of_very_wide_rows():
     for name, got in (("y", y), ("dx", dx), ("dweight", dw)):
         value, bound = want[name]
         assert ((got.detach().double() - value).abs() <= bound).all(), name
+
+
+@pytest.mark.parametrize("N", [8, 1000, 5000, 20000])
+@pytest.mark.parametrize("dtype", [0, 2])
+def test_layer_norm_backward_without_rows_from_c(dtype, N):
+    """No rows, an address for dx all the same: the parameters' gradients are zeros."""
+    lib = _lib.lib()
+    size = 4 if dtype == 0 else 2
+    room = torch.full((8, N), 7.0, device="cuda")
+    scratch = torch.full((int(lib.gfpp_layer_norm_backward_scratch_floats(0, N)),), math.nan, device="cuda")
+    p = [ctypes.c_void_p(room[i].data_ptr()) for i in range(8)]
+    torch.cuda.synchronize()
+    assert N * size % 16 == 0
+    stream = ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
+    assert lib.gfpp_layer_norm_backward(p[0], N, p[1], N, p[2], 0, p[3], p[4], 0, N, dtype, p[5], p[6], p[7], ctypes.c_void_p(scratch.data_ptr()), stream) == 0, lib.gfpp_last_error()
+    assert not room[6:].any() and (room[:6] == 7.0).all()
