@@ -99,7 +99,7 @@ def build(verbose=False):
         obj_cpp = os.path.join(OUT, name + ".bindings.o")
         common = ["-O3", "-std=c++17", "-fPIC", "-w", f"-DTORCH_EXTENSION_NAME={name}", "-I", SHIM] + defs + inc
         script = " && ".join(" ".join(c) for c in (
-            [HIPCC, "-x", "hip", f"--offload-arch={ARCH}"] + common + extra + ["-c", src_cu, "-o", obj_cu],
+            [HIPCC, "-x", "hip", f"--offload-arch={ARCH}", "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"] + common + extra + ["-c", src_cu, "-o", obj_cu],
             [HIPCC, "-x", "c++"] + common + ["-c", src_cpp, "-o", obj_cpp],
             [HIPCC, f"--offload-arch={ARCH}", "-shared", "-fPIC", obj_cu, obj_cpp, "-o", so] + link,
             ["rm", "-f", obj_cu, obj_cpp]))

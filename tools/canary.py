@@ -3,7 +3,7 @@ loads, shuffles, dot products -- each repetition compared with the wavefront's o
 
 STATUS: written at the end of round 6 and compiled for gfx950; GPU access closed before it ran once (docs/LAB_NOTEBOOK.md).  Treat it as unverified.
 
-    hipcc --offload-arch=gfx950 -O3 -std=c++17 -fPIC -shared -o build/probe/libcanary.so tools/probe/canary.hip      (here; the .so travels with gpurun)
+    hipcc --offload-arch=gfx950 -O3 -std=c++17 -Xclang -target-feature -Xclang -packed-fp32-ops -fPIC -shared -o build/probe/libcanary.so tools/probe/canary.hip      (here; the .so travels with gpurun)
     python tools/canary.py [launches] [iters per launch] [workgroups]
 """
 import ctypes

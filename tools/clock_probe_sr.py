@@ -17,7 +17,7 @@ from genefaceplusplus_amd.radnerfs.superres import Superresolution  # noqa: E402
 
 src = os.path.join(ROOT, "tools", "probe", "clock_probe.hip")
 so = "/tmp/clock_probe.so"
-subprocess.check_call(["/opt/rocm/bin/hipcc", "--offload-arch=gfx950", "-O2", "-shared", "-fPIC", src, "-o", so])
+subprocess.check_call(["/opt/rocm/bin/hipcc", "--offload-arch=gfx950", "-O2", "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops", "-shared", "-fPIC", src, "-o", so])
 lib = ctypes.CDLL(so)
 lib.clock_probe_launch.argtypes = [ctypes.c_void_p, ctypes.c_uint32, ctypes.c_uint32, ctypes.c_void_p]
 dev = torch.device("cuda:0")

@@ -3,7 +3,7 @@
 // products + v_permlane32_swap -- and compare every repetition with the FIRST one (same wavefront, same registers, same inputs: any difference is a transient fault).
 // tools/canary.py runs it on one stream while another stream keeps the SR stage in flight.
 //
-//   hipcc --offload-arch=gfx950 -O3 -std=c++17 -fPIC -shared -o build/probe/libcanary.so tools/probe/canary.hip
+//   hipcc --offload-arch=gfx950 -O3 -std=c++17 -Xclang -target-feature -Xclang -packed-fp32-ops -fPIC -shared -o build/probe/libcanary.so tools/probe/canary.hip
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
