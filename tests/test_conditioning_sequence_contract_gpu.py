@@ -245,3 +245,44 @@ def test_layer_norm_backward_without_rows_from_c(dtype, N):
     stream = ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
     assert lib.gfpp_layer_norm_backward(p[0], N, p[1], N, p[2], 0, p[3], p[4], 0, N, dtype, p[5], p[6], p[7], ctypes.c_void_p(scratch.data_ptr()), stream) == 0, lib.gfpp_last_error()
     assert not room[6:].any() and (room[:6] == 7.0).all()
+
+
+# ---- arguments in company --------------------------------------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS)
+@pytest.mark.parametrize("Tq,Tk,start,left,right,sinks,lengths", [(70, 200, 100, 30, 0, 3, (200, 120, 0)), (64, 150, 60, 20, 10, 0, (61, 150, 124)), (90, 64, 10, None, 0, 2, (64, 11, 40)),
+                                                                  (300, 330, 30, 70, 0, 5, (330, 200, 31))])
+def test_chunks_of_padded_streams(Tq, Tk, start, left, right, sinks, lengths, dtype):
+    """Queries that are some of the tokens of sequences of several lengths."""
+    B, Hq, Hk, D = 3, 4, 2, 40
+    q, k, v, dout = (rand(s, B, t, h, D, dtype=dtype) for s, (t, h) in enumerate(((Tq, Hq), (Tk, Hk), (Tk, Hk), (Tq, Hq))))
+    how = dict(left=left, right=right, sinks=sinks, q_start=start)
+    want = ref.attention(*(t.cpu() for t in (q, k, v, dout)), lengths=lengths, **how)
+    leaves = [t.detach().requires_grad_(True) for t in (q, k, v)]
+    out = window_attention(*leaves, lengths=torch.tensor(lengths).cuda(), **how)
+    for name, got in zip(("out", "dq", "dk", "dv"), (out, *torch.autograd.grad(out, leaves, dout))):
+        ref.close(got, want[name], name)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS)
+def test_step_of_strided_tokens(dtype):
+    """Queries, keys and values out of one projection, every other head, one head for all, features apart."""
+    B, Hq, Hk, D, slots, sinks = 3, 4, 2, 32, 40, 2
+    q, k, v = rand(0, B, Hq, D, dtype=dtype), rand(1, B, Hk, D, dtype=dtype), rand(2, B, Hk, D, dtype=dtype)
+    pos = torch.tensor([5, 100, 39], dtype=torch.int32).cuda()
+    fresh = lambda: (rand(3, B, slots, Hk, D, dtype=dtype), rand(4, B, slots, Hk, D, dtype=dtype))  # noqa: E731
+    ck, cv = fresh()
+    want = (window_attention_step(q, k, v, ck, cv, pos, sinks), ck, cv)
+    packed = torch.cat((q, k, v), 1)
+    apart = [torch.stack((t, t), 2).view(B, -1, D)[:, ::2] for t in (q, k, v)]
+    odd = [torch.nn.functional.pad(t, (1, 2))[..., 1:1 + D] for t in (q, k, v)]
+    features = [t.transpose(1, 2).contiguous().transpose(1, 2) for t in (q, k, v)]
+    for a, b, c in ((packed[:, :Hq], packed[:, Hq:Hq + Hk], packed[:, Hq + Hk:]), apart, odd, features):
+        assert torch.equal(a, q) and torch.equal(b, k) and torch.equal(c, v)
+        ck, cv = fresh()
+        got = (window_attention_step(a, b, c, ck, cv, pos, sinks), ck, cv)
+        assert all(torch.equal(x, y) for x, y in zip(got, want))
+    one = q[:, :1].expand(B, Hq, D)
+    ck, cv = fresh()
+    out = window_attention_step(one, k, v, ck, cv, pos, sinks)
+    ck, cv = fresh()
+    assert torch.equal(out, window_attention_step(one.contiguous(), k, v, ck, cv, pos, sinks))
