@@ -246,9 +246,9 @@ __device__ __forceinline__ void level_fast_issue(const float (&u)[D], const floa
 
 template <int D>
 __device__ __forceinline__ void level_fast_finish(const LevelGathers<D> &g, float (&out)[2]) {
-    // corner weights and accumulation on packed fp32 pairs (v_pk_mul_f32 / v_pk_fma_f32): (w0, w1) = ((1 - fx) * yf * zf, fx * yf * zf) with the
-    // products in grid_level_lookup's order, so the (1 - fx, fx) * yf halves are shared by the two z planes -- 6 packed multiplies per 3-D level
-    // instead of 16 scalar ones, same bits
+    // corner weights and accumulation on pairs (an fp32 instruction per half: the packed ones are off, Makefile): (w0, w1) = ((1 - fx) * yf * zf, fx * yf * zf) with the
+    // products in grid_level_lookup's order, so the (1 - fx, fx) * yf halves are shared by the two z planes -- 6 pairs of multiplies per 3-D level
+    // instead of 16 single ones, same bits
     constexpr int kPairs = 1 << (D - 1);
     typedef float f32x2 __attribute__((ext_vector_type(2)));
     const f32x2 wx = {1.0f - g.frac[0], g.frac[0]};
@@ -315,7 +315,7 @@ __device__ __forceinline__ void level_block_finish(const BlockGathers<D> &g, flo
     typedef float f32x2 __attribute__((ext_vector_type(2)));
     const f32x2 wx = {1.0f - g.frac[0], g.frac[0]};
     // the four x-y corner weights of the cell once, in fp16 (they are the same in both z planes); the z interpolation happens on the two planes' fp32 sums:
-    // 2 packed multiplies + 2 conversions + 8 dot products + 2 packed blend operations per 3-D level (6 + 4 + 8 with the z weight folded into the corner weights)
+    // 2 pairs of multiplies + 2 conversions + 8 dot products + 2 pairs of blend operations per 3-D level (6 + 4 + 8 with the z weight folded into the corner weights)
     const gfpp_h2 h0 = __builtin_convertvector(wx * (1.0f - g.frac[1]), gfpp_h2), h1 = __builtin_convertvector(wx * g.frac[1], gfpp_h2);
     typedef _Float16 h8 __attribute__((ext_vector_type(8)));
     f32x2 plane[D == 3 ? 2 : 1];

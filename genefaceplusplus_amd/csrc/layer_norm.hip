@@ -4,12 +4,14 @@
 //   g = dy w:   dx = rstd (g - mean(g) - xhat mean(g xhat)),   dw = sum_rows dy xhat,   db = sum_rows dy
 //
 // Bound by memory: a forward pass reads x and writes y, a backward pass reads x and dy and writes dx.  A row is therefore held in registers between its
-// statistics and its output (the variance is that of the centred values, not E x^2 - mean^2), by one wavefront or one workgroup of 256 (rows up to 8 192
-// elements); longer rows are read again, out of the L2.  Statistics, both row sums of the backward pass and the column sums are fp32 for every type; the outputs
+// statistics and its output (the variance is that of the centred values, not E x^2 - mean^2), by one wavefront or one workgroup of 256.  Forward: rows of up to 8 192 elements,
+// fp32 rows in vectors up to 4 096; backward, which holds two rows and the column sums: up to 4 096, fp32 rows in vectors up to 2 048.  Longer rows are read again out of the
+// caches, three times in the forward pass, twice for dx, and once more from memory for the column sums (8 192 x 8 192 bf16: forward 50 us, backward 209; fp32 157 and 339;
+// 13 000 x 4 096 bf16, still in registers: 37 and 108).  Statistics, both row sums of the backward pass and the column sums are fp32 for every type; the outputs
 // are rounded once.  The column sums of dw / db stay in registers over the rows of a workgroup, leave as one partial row per workgroup and are added in a fixed
 // order by a second launch: no atomics, the same bits every time.
-// Measured: 13 000 x 1 024 bf16 with fp32 parameters: forward 12.8 us (53 MB, 4.2 TB/s), backward 21.9 (80 MB, 3.6 TB/s) and 4.0 for the column sums; 65 537 x 204 fp32: forward
-// 24.5 us (107 MB, 4.4 TB/s), backward 28.9 (160 MB, 5.5 TB/s) and 4.0.  Rows that 16-byte vectors do not divide go one element at a time: 24.7 and 36.3, 32.2 and 47.0.
+// Measured: 13 000 x 1 024 bf16 with fp32 parameters: forward 12.5 us (53 MB, 4.3 TB/s), backward 21.2 (80 MB, 3.8 TB/s) and 3.9 for the column sums; 65 537 x 204 fp32: forward
+// 23.9 us (107 MB, 4.5 TB/s), backward 28.8 (160 MB, 5.6 TB/s) and 3.9.  Rows that 16-byte vectors do not divide go one element at a time: 24.7 and 36.3, 32.2 and 47.0.
 // One row of 1 024: 2.7 us, a launch.
 #include <algorithm>
 
@@ -417,7 +419,8 @@ __global__ __launch_bounds__(1024) void k_layer_norm_cols(const float *__restric
 constexpr uint32_t kLnMostGrid = 32768;
 
 // workgroups of the backward pass = partial rows: four per CU (65 537 x 204 fp32: 28.5 us, two per CU 37.7; 13 000 x 1 024 bf16: 21.9, six per CU 28.9), no more than there
-// are rows to take
+// are rows to take.  Four rows a workgroup are counted up to 1 024 columns; fp32 rows of 513 to 1 024 take a whole workgroup each and so share one by fours.  Measured at these two
+// widths: from 4 096 columns on the partial rows weigh as much as the data (3 250 x 4 096 bf16: backward 68 us for 80 MB).
 static uint32_t ln_bwd_groups(uint64_t M, uint32_t N) {
     const uint64_t rpw = N <= 1024 ? 4 : 1;
     const uint64_t want = (M + rpw - 1) / rpw;

@@ -8,7 +8,7 @@
 //
 // Bound by memory: every element is read and written once.  A workgroup takes a few tokens, computes their cosines and sines once into LDS (they are shared by all
 // heads of both tensors: queries and keys go through in ONE launch) and streams the heads in 16-byte vectors.
-// Measured: 16 384 tokens x (16 + 4) heads x 128 bf16: 34 us (168 MB, 4.9 TB/s; one element at a time: 87); 3 x 1 023 x 9 x 40 fp32: 5.4 us (8.8 MB); 8 tokens: 3.6 us, a launch.
+// Measured: 16 384 tokens x (16 + 4) heads x 128 bf16: 34 us (168 MB, 4.9 TB/s; one element at a time, which is what pairs that do not fill 16-byte vectors take: 87); 3 x 1 023 x 9 x 40 fp32: 5.4 us (8.8 MB); 8 tokens: 3.4 us, a launch.
 #include "gfpp_common.h"
 
 namespace gfpp {

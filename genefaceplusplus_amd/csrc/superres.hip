@@ -101,9 +101,9 @@ __device__ __forceinline__ float sr_act(float v, float gain, float clamp) {
     v = (v >= 0.0f ? v : 0.2f * v) * gain;
     return fminf(fmaxf(v, -clamp), clamp);
 }
-// The same function on two values in packed fp32 instructions, bit for bit: v g for v >= 0 and (0.2 v) g for v < 0 are both computed (the same roundings as the
-// select) and the larger one IS the selected one (v >= 0: v g >= 0.2 v g; v < 0: the other way round); the clamp is one median-of-three.  4.5 vector
-// instructions per value instead of 8.4 -- the epilogues of these kernels are vector-ALU bound (tools/sr_phase.py), not matrix bound.
+// The same function on two values, bit for bit: v g for v >= 0 and (0.2 v) g for v < 0 are both computed (the same roundings as the
+// select) and the larger one IS the selected one (v >= 0: v g >= 0.2 v g; v < 0: the other way round); the clamp is one median-of-three.  5 vector
+// instructions per value instead of 8.4 (without packed fp32, which is off: Makefile) -- the epilogues of these kernels are vector-ALU bound (tools/sr_phase.py), not matrix bound.
 typedef float sr_f32x2 __attribute__((ext_vector_type(2)));
 __device__ __forceinline__ sr_f32x2 sr_act2(sr_f32x2 v, float gain, float clamp) {
     const sr_f32x2 pos = v * gain, neg = (v * 0.2f) * gain;

@@ -7,7 +7,9 @@
 // values go through LDS, double-buffered, the tile after next in flight in registers, one barrier per tile.  S^T = K Q^T puts a query's scores into ONE lane pair: the
 // row maximum and sum are register arithmetic, the probabilities are the operand of O^T = V^T P^T without leaving their registers, and the accumulators are rescaled
 // by one factor per lane -- only when a maximum has grown by more than 2^8, since exp2(s - m) with a slightly old m is as exact.
-// Probabilities are rounded to the operand type (16-bit modes) for the matrix instruction; l sums the unrounded ones in fp32.
+// Probabilities are rounded to the operand type (16-bit modes) for the matrix instruction; l sums the unrounded ones in fp32.  That is a choice: against 64 bits the output is off by
+// 2.4e-3 of its norm (bf16, window 1 024) where its own rounding alone is 1.7e-3.  The matrix pipe takes fp32 operands at an eighth of the rate, and as a rounded value and its
+// remainder (done where it shows: window_attn_device.h, the two-part rule) half as many products again.
 #include "window_attn_device.h"
 
 namespace gfpp {
@@ -22,8 +24,9 @@ constexpr int wa_bn() { return FEW || (sizeof(T) == 4 && DP == 128) || (sizeof(T
 // WAVES 1: 32 queries a workgroup instead of 128, for few keys and a grid that would leave CUs empty (296 x 4 heads x 16, window 8, fp32: 8.5 us, with 128 queries 13.8).
 // VEC: 16-byte accesses (wa_vectors); one element at a time otherwise (13 000 x 8 heads x 64, window 1 024: 69 and 180 us).
 //
-// Bound by the barrier of every tile and the tiles' way through LDS, then by the matrix pipe.  Measured (bf16): 16 384 x 16 heads on 4 x 128, window 2 049: 313 us (266 GFLOP,
-// 0.85 PFLOP/s); 13 000 x 8 on 2 x 64, window 1 024, 4 sinks: 69 us (26 GFLOP, 0.38 PFLOP/s: at 64 features every 64 products come with an exponential).
+// No unit is full: what is left is waiting (a third of the wavefronts' time for data and barriers, near a third for their turn to issue).  Measured (bf16): 16 384 x 16 heads on 4 x 128,
+// window 2 049: 295 us (266 GFLOP, 0.90 PFLOP/s; of the CUs' cycles the matrix pipe is busy in 45 %, the LDS in 28 %); 13 000 x 8 on 2 x 64, window 1 024, 4 sinks: 68 us (26 GFLOP,
+// 0.39 PFLOP/s; 26 and 20 %: at 64 features every 64 products come with an exponential).
 template <typename T, int DP, bool VEC, bool FEW, int HEADS, int WAVES>
 __global__ __launch_bounds__(64 * WAVES * HEADS, WAVES == 1 ? 1 : (sizeof(T) == 2 ? (DP <= 64 && VEC ? (FEW ? 3 : 4) : (VEC || HEADS == 2 ? 2 : 1)) : 1)) void k_window_attn(WaArgs a) {
     constexpr int BN = wa_bn<T, DP, FEW>(), ROWS = 32 * WAVES, NS = DP / 16, NT = DP / 32, NSUB = BN / 32, PK = wa_pitch_row<T, DP>(), PV = wa_pitch_col<T, DP>();

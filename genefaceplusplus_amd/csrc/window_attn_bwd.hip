@@ -7,7 +7,8 @@
 // atomics: every gradient is summed by one workgroup in a fixed order, the heads of a group one after the other.  The tiles that hold sinks are seen by ALL later
 // queries; their queries are cut into slices that leave fp32 partial sums, which a third launch adds in the slices' order.
 // delta is a matrix product's diagonal, taken by the instructions that compute dout . v: where a query sees one key only, out = v and ds is exactly zero.
-// p and ds are rounded to the operand type (16-bit modes) for the matrix instruction; every sum is fp32.
+// p and ds are rounded to the operand type (16-bit modes) for the matrix instruction; every sum is fp32.  A choice, as in the forward pass: the gradients' error against 64 bits grows
+// from 1.7e-3 of their norm (their own rounding) to 2.4e-3 (bf16), and two parts each would take half as many products again for dk and dv, a third for dq.
 #include "window_attn_device.h"
 
 namespace gfpp {
@@ -17,8 +18,9 @@ int wa_arguments(const char *what, WaArgs &a, const int64_t *strides, int n_tens
 bool wa_vectors(const WaTensor &t, int D, size_t size);
 
 // dq of 128 queries of one head, 32 a wavefront, over tiles of keys and values in LDS; s and dout . v both as K Q^T and V dout^T, so that ds is the operand of dq^T += K^T ds^T
-// without leaving its registers.  Measured (bf16): 16 384 x 16 heads on 4 x 128, window 2 049: 425 us (400 GFLOP, 0.94 PFLOP/s; two heads of a group on one workgroup, as in the
-// forward pass: no difference); 13 000 x 8 on 2 x 64, window 1 024, 4 sinks: 84 us (39 GFLOP, 0.47 PFLOP/s).
+// without leaving its registers.  Measured (bf16): 16 384 x 16 heads on 4 x 128, window 2 049: 406 us (400 GFLOP, 0.98 PFLOP/s; matrix pipe busy in 49 % of the CUs' cycles,
+// LDS in 41 %, a fifth of that bank conflicts; two heads of a group on one workgroup, as in the forward pass: no difference); 13 000 x 8 on 2 x 64, window 1 024, 4 sinks: 84 us
+// (39 GFLOP, 0.47 PFLOP/s; 36 and 31 %).
 template <typename T, int DP, bool VEC>
 __global__ __launch_bounds__(kWaThreads, sizeof(T) == 2 && (VEC || DP <= 64) ? 2 : 1) void k_window_attn_dq(WaArgs a) {
     constexpr int BN = DP == 128 ? 32 : 64, NS = DP / 16, NT = DP / 32, PK = wa_pitch_both<T, DP>(), PV = wa_pitch_row<T, DP>();
@@ -150,8 +152,9 @@ __global__ __launch_bounds__(kWaThreads, sizeof(T) == 2 && (VEC || DP <= 64) ? 2
 // Three tiles are held: the one being stored, the one that is read by the first wavefronts and the one that is read by the second.  AHEAD (16-bit heads of 33 to 64
 // features): the second take their product with dout a tile early and hold it, so that two tiles of dout are enough and three workgroups fit a CU.
 // Work items: first the slices of the tiles with sinks (a.splits each, partial sums), then the other tiles.
-// Bound by the barrier of every tile and the tiles' way through LDS.  Measured (bf16): 16 384 x 16 heads on 4 x 128, window 2 049: 787 us (533 GFLOP, 0.68 PFLOP/s);
-// 13 000 x 8 on 2 x 64, window 1 024, 4 sinks: 155 us (53 GFLOP, 0.34 PFLOP/s).  128 keys a workgroup instead of 64 took within 1.5 % of that at 128 features and 3 to 20 %
+// Neither the matrix pipe nor the LDS is full; the wavefronts of a pair wait for one another at every tile's barrier.  Measured (bf16): 16 384 x 16 heads on 4 x 128, window 2 049:
+// 725 us (533 GFLOP, 0.74 PFLOP/s; matrix pipe busy in 33 % of the CUs' cycles, LDS in 44 %, a fifth of that bank conflicts); 13 000 x 8 on 2 x 64, window 1 024, 4 sinks: 153 us
+// (53 GFLOP, 0.35 PFLOP/s; 18 and 30 %: 430 workgroups where 768 fit).  128 keys a workgroup instead of 64 took within 1.5 % of that at 128 features and 3 to 20 %
 // more at 64 and fewer (16 384 x 16 heads x 64, window 301: dq, dk and dv together 289 us against 237, and 206 with AHEAD).
 constexpr int kWaBq = 32, kWaKeys = 64, kWaPairs = kWaKeys / 32;
 template <typename T, int DP, bool VEC>

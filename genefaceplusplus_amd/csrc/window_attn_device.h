@@ -14,7 +14,7 @@
 
 namespace gfpp {
 
-constexpr int kWaThreads = 256, kWaRows = 128;      // four wavefronts of 32 queries (forward, dq); dk and dv: 128 keys, eight wavefronts
+constexpr int kWaThreads = 256, kWaRows = 128;      // four wavefronts of 32 queries (forward, dq); dk and dv: 64 keys, two wavefronts for every 32
 
 template <int N>
 struct WaInt {
@@ -37,8 +37,8 @@ struct WaArgs {
     uint32_t sink_tiles, splits;
 };
 
-// two query heads per workgroup: an even group, and enough workgroups left to fill the chip (16 384 x 16 heads on 4 x 128, window 2 049, bf16, forward: 313 to 329 us,
-// one head each 342; the backward kernels do not gain)
+// two query heads per workgroup: an even group, and enough workgroups left to fill the chip (16 384 x 16 heads on 4 x 128, window 2 049, bf16, forward, in turn on one card: 313 to
+// 329 us, one head each 342; the backward kernels do not gain)
 inline bool wa_pair_heads(const WaArgs &a, uint64_t grid) { return a.G % 2 == 0 && grid / 2 >= (uint64_t)cu_count(); }
 
 // Workgroups are dealt out to the 8 XCDs in turn, each with an L2 of its own: the work items of one XCD are made neighbours (which read the same keys or

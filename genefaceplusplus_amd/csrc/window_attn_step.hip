@@ -3,13 +3,14 @@
 // The cache of a stream holds its first `sinks` tokens and its last W = slots - sinks ones; the token at position n lives in slot  n < sinks ? n : sinks +
 // (n - sinks) mod W.  A step writes the new key and value into their slot and attends over the min(n + 1, slots) slots that are filled: exactly the keys that
 // window_attn.hip's rule shows position n with left = W - 1, right = 0.  Softmax does not ask for an order, so the ring is read as it lies.
+// A negative position leaves its stream as it is.
 //
 // Bound by memory: the filled slots are read once for all query heads of a group.  The group's heads are the 32 columns of the matrix products (window_attn_device.h's
 // layout): keys come straight from memory as row fragments, values pass through a wavefront's own 32 rows of LDS for the transposing read.  A wavefront takes every
 // fourth tile of 32 slots of its workgroup's stretch, the next tile in flight in registers; the four partial softmaxes meet in LDS.  Few streams: the
 // slots of a stream are split over several workgroups, whose partial results a second launch joins.
 // Probabilities enter the products as a rounded value and its rounded remainder, so that the output carries its own rounding alone.
-// Measured (bf16): 64 streams x 32 heads on 8 x 128, 4 100 slots (1.08 GB): 184 us (5.8 TB/s; a copy of 2 GiB moves 5.2) and 7 for the join; one stream x 8 on 2 x 64, 260 slots:
+// Measured (bf16): 64 streams x 32 heads on 8 x 128, 4 100 slots (1.08 GB): 180 us (6.0 TB/s; a copy of 2 GiB moves 5.2) and 7 for the join; one stream x 8 on 2 x 64, 260 slots:
 // 6.3 us, a launch's latency and four dependent trips to memory.  One element at a time (unaligned rows) takes 1 000 and 23 us.
 // The row of the new token is taken from the arguments by whoever reads that slot, and written by one wavefront: no order between workgroups is needed.
 #include "window_attn_device.h"

@@ -293,7 +293,8 @@ def rotary_embed(x, positions, frequencies, sections, interleaved=False):
 class RotaryEncoder(nn.Module):
     """rotary_embed with its frequencies: theta^(-i / n) over the n pairs of every axis, or over all P pairs counted through (joint).
 
-    dim: head width; sections: pairs of every axis (their sum at most dim // 2, the rest of a head passes through).  No parameters."""
+    dim: head width; sections: pairs of every axis (their sum at most dim // 2, the rest of a head passes through).  No parameters; the frequencies move with
+    the module (Module.to) or with its first call on a device, which must not be a captured one."""
 
     def __init__(self, dim, sections, theta=10000.0, interleaved=False, joint=False):
         super().__init__()

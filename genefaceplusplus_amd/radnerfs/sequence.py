@@ -5,7 +5,8 @@ a conditioning network over whole clips (thousands of frames, forward and backwa
 them are in encoders.py.  Hand-written HIP kernels through the C ABI (csrc/layer_norm.hip, window_attn*.hip); float32, float16 and bfloat16, sums in float32.
 
 Tensors live on one GPU, nothing is moved silently; kernels run on torch's current stream of that GPU.  Gradients are first derivatives only, summed in a fixed
-order (the same bits every time).  Argument checks, allocation and the autograd nodes are compiled (csrc/sequence_torch.cpp)."""
+order (the same bits every time); tangents of forward mode and tracers (torch.jit.trace, make_fx), which would not see the kernels, are refused.  Argument checks,
+allocation and the autograd nodes are compiled (csrc/sequence_torch.cpp)."""
 import ctypes
 import importlib
 import os
@@ -74,8 +75,8 @@ def window_attention(q, k, v, left=None, right=0, sinks=0, lengths=None, scale=N
     """softmax(scale q k^T) v over the keys that each query sees; differentiable in q, k and v.
 
     q [B, Tq, Hq, D], k and v [B, Tk, Hk, D], Hq a multiple of Hk (query head h reads key head h // (Hq // Hk)), D up to 128 -> [B, Tq, Hq, D].
-    The query at position p = q_start + i sees key j iff ``j <= p + right and (j >= p - left or j < sinks)``; left / right None: no end on that side.
-    q_start: Tk - Tq by default (the queries are the last tokens).  lengths: [B] int32 / int64 on the GPU, tokens of every sequence: what lies behind is neither
+    The query at position p = q_start + i sees key j iff ``j <= p + right and (j >= p - left or j < sinks)``; left / right None: no end on that side.  Queries are tokens of
+    the sequence: one at p >= Tk is behind its end and sees nothing.  q_start: Tk - Tq by default (the queries are the last tokens).  lengths: [B] int32 / int64 on the GPU, tokens of every sequence: what lies behind is neither
     read nor seen, its output rows and gradients are zero, as are those of a query that sees nothing.  Within its length a sequence has to be finite.
     scale: D ** -0.5 by default."""
     return (_ops or ops()).window_attention(q, k, v, left, right, sinks, lengths, scale, q_start)
@@ -87,7 +88,8 @@ def window_attention_step(q, k, v, cache_k, cache_v, positions, sinks=0, scale=N
     q [B, Hq, D], k and v [B, Hk, D] -> [B, Hq, D]; cache_k, cache_v [B, slots, Hk, D] (any strides with a dense last axis) hold a stream's first `sinks` tokens
     and its last W = slots - sinks ones, the token at position n in slot ``n if n < sinks else sinks + (n - sinks) % W``.  positions: [B] int32 / int64 on the GPU, the
     new tokens' positions; a negative one leaves its stream as it is (output zeros).  The result is row n of window_attention(left=W - 1, right=0, sinks=sinks)
-    over the whole stream.  Serving only: no gradients.  Positions and caches are read on the GPU, so a captured graph of steps can be replayed."""
+    over the whole stream.  No two slots may share memory, and q, k, v may not lie in the caches.  Serving only: no gradients; the caches count as modified in place (a
+    backward pass that has kept them raises).  Positions and caches are read on the GPU, so a captured graph of steps can be replayed."""
     return (_ops or ops()).window_attention_step(q, k, v, cache_k, cache_v, positions, sinks, scale)
 
 

@@ -847,7 +847,9 @@ int gfpp_sr_forward(const gfpp_sr_model *model, const gfpp_sr_ws *ws, const floa
  * Section C -- sequence operators of the conditioning stage (beside AudioNet / AudioAttNet, cond_encoder.py:98-180, which smooth windows of 1 .. 16 frames; the
  * reference has no native counterpart).  dtype: GFPP_F32 / GFPP_F16 / GFPP_BF16, the type of every tensor that is not named otherwise; statistics, softmax sums
  * and reductions are fp32.  Strides are in elements; the last axis of every tensor has stride 1; rows may start anywhere (16-byte vectors where every pointer and
- * stride allows them, single elements otherwise).  `strides`, `sections` are HOST arrays.  Scratch is the caller's, per call; nothing is kept between calls.
+ * stride allows them, single elements otherwise).  `strides`, `sections` are HOST arrays.  Scratch is the caller's, per call; nothing is kept between calls.  A call
+ * whose grid would reach 2^32 threads (rotary: 2^24 tokens and more, by its pairs; attention: 2^24 tiles of 128 queries x Hq x B or of 64 keys x Hk x B; step: 2^24
+ * (stream, key head) pairs, by its slots) is GFPP_EINVAL.
  * ---------------------------------------------------------------------------------------------------------- */
 
 /* Layer norm over the last axis in front of a conditioning network's layers (cond_encoder.py:98-143 has none): y[m] = (x[m] - mean) / sqrt(var + eps) * weight +
@@ -873,7 +875,7 @@ int gfpp_rotary(const void *x0, const int64_t *x0_strides, uint32_t heads0, void
 /* Attention with a sliding window and visible first tokens over a conditioning sequence (AudioAttNet's weighted window, cond_encoder.py:146-180, for sequences of any
  * length): out[b, i, h] = sum_j softmax_j(scale q[b, i, h] . k[b, j, h / G]) v[b, j, h / G], G = Hq / Hk, over the keys j that the query at position p = q_start + i
  * sees:  j < n and p < n and j <= p + right and (j >= p - left or j < sinks),  n = min(lengths[b], Tk) (lengths NULL: Tk).  A query that sees nothing gives
- * zeros.  out_low: NULL, or where gfpp_window_attn_two_part says so (16-bit types, few visible keys) a tensor with out's strides that takes what out's rounding left,
+ * zeros, one behind the keys' end (p >= n) among them.  out_low: NULL, or where gfpp_window_attn_two_part says so (16-bit types, few visible keys) a tensor with out's strides that takes what out's rounding left,
  * for the backward pass.  q, out [B, Tq, Hq, D]; k, v [B, Tk, Hk, D]; strides: {B, T, H} of q, k, v, out; D 1 .. 128.  lse [B, Hq, Tq] f32 for the backward pass, or NULL.
  * Rows behind a sequence's length are not read (they may hold anything); within it keys and values have to be finite. */
 int gfpp_window_attn_forward(const void *q, const void *k, const void *v, void *out, void *out_low, float *lse, const int64_t *strides, uint32_t B, uint32_t Tq, uint32_t Tk,
@@ -882,7 +884,8 @@ int gfpp_window_attn_forward(const void *q, const void *k, const void *v, void *
 /* (cond_encoder.py:146-180, as above) */
 int gfpp_window_attn_two_part(uint32_t Tk, int32_t left, int32_t right, int32_t sinks, int dtype);
 /* Its backward pass (cond_encoder.py:146-180, as above): dq, dk, dv from dout, the forward pass' inputs, out and lse.  strides: {B, T, H} of q, k, v, out, dout, dq,
- * dk, dv.  Every row of dq, dk and dv is written (zeros behind a sequence's length).  No atomics: the same bits every time. */
+ * dk, dv.  Every row of dq, dk and dv is written (zeros behind a sequence's length).  No atomics: the same bits every time.  Scratch: B Hq Tq floats, and with sinks
+ * at most 4 096 x 128 D more. */
 int gfpp_window_attn_backward(const void *q, const void *k, const void *v, const void *out, const void *out_low, const void *dout, const float *lse, void *dq, void *dk, void *dv,
                               float *scratch, const int64_t *strides, uint32_t B, uint32_t Tq, uint32_t Tk, uint32_t Hq, uint32_t Hk, uint32_t D, int32_t left,
                               int32_t right, int32_t sinks, int32_t q_start, const int32_t *lengths, float scale, int dtype, gfpp_stream_t stream);
@@ -893,7 +896,7 @@ unsigned long long gfpp_window_attn_backward_scratch_floats(uint32_t B, uint32_t
 /* One new token per stream (AudioAttNet's weighted window, cond_encoder.py:146-180, for a live stream): stream b's token at positions[b] (int32, or int64 with
  * positions64) writes k[b], v[b] [Hk, D] into its slot of cache_k, cache_v [B, slots, Hk, D] -- n < sinks ? n : sinks + (n - sinks) mod (slots - sinks) -- and
  * out[b] [Hq, D] is its attention over the min(n + 1, slots) filled slots: gfpp_window_attn_forward's row n with left = slots - sinks - 1, right = 0.  A negative
- * position: the stream is left as it is and its output is zeros.  strides: q {B, H}, k {B, H}, v {B, H}, cache_k {B, slot, H}, cache_v {B, slot, H}, out {B, H}. */
+ * position: the stream is left as it is and its output is zeros.  No two slots may share memory, within a cache or between the two, and q, k, v may not lie in them.  strides: q {B, H}, k {B, H}, v {B, H}, cache_k {B, slot, H}, cache_v {B, slot, H}, out {B, H}. */
 int gfpp_window_attn_step(const void *q, const void *k, const void *v, void *cache_k, void *cache_v, const void *positions, int positions64, void *out,
                           const int64_t *strides, uint32_t B, uint32_t Hq, uint32_t Hk, uint32_t D, uint32_t slots, uint32_t sinks, float scale, int dtype,
                           float *scratch, gfpp_stream_t stream);
