@@ -286,3 +286,45 @@ def test_step_of_strided_tokens(dtype):
     out = window_attention_step(one, k, v, ck, cv, pos, sinks)
     ck, cv = fresh()
     assert torch.equal(out, window_attention_step(one.contiguous(), k, v, ck, cv, pos, sinks))
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS)
+@pytest.mark.parametrize("B,Tq,Tk", [(2, 5, 0), (2, 0, 9), (0, 5, 9), (2, 0, 0)])
+@pytest.mark.parametrize("D,sinks", [(64, 0), (64, 3), (5, 1)])
+def test_attention_of_nothing(dtype, B, Tq, Tk, D, sinks):
+    """No keys, no queries, no sequences: outputs and gradients of the right shapes, all zeros."""
+    q, k, v, dout = (rand(s, B, t, h, D, dtype=dtype) for s, (t, h) in enumerate(((Tq, 4), (Tk, 2), (Tk, 2), (Tq, 4))))
+    leaves = [t.requires_grad_(True) for t in (q, k, v)]
+    for lengths in (None, torch.full((B,), Tk).cuda()):
+        out = window_attention(*leaves, left=3, sinks=sinks, lengths=lengths, q_start=0)
+        for t, like in zip((out, *torch.autograd.grad(out, leaves, dout)), (q, q, k, v)):
+            assert t.shape == like.shape and t.dtype == dtype and not t.any()
+
+
+def test_lengths_of_a_captured_pass_are_read_at_every_replay():
+    """Lengths that change between the replays, in either type; what lies behind them stays zero."""
+    B, T, H, D = 3, 90, 2, 32
+    q, k, v, dout = (rand(s, B, T, H, D) for s in range(4))
+    for kind in (torch.int32, torch.int64):
+        lengths = torch.tensor((90, 17, 0), dtype=kind).cuda()
+        leaves = [t.clone().requires_grad_(True) for t in (q, k, v)]
+
+        def run():
+            out = window_attention(*leaves, left=20, right=2, sinks=1, lengths=lengths)
+            return (out.detach(), *torch.autograd.grad(out, leaves, dout))
+
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            run()
+        torch.cuda.current_stream().wait_stream(side)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            kept = run()
+        for now in ((90, 17, 0), (0, 90, 33), (5, 64, 89), (200, -3, 1)):
+            lengths.copy_(torch.tensor(now))
+            graph.replay()
+            torch.cuda.synchronize()
+            got = [t.clone() for t in kept]
+            for a, b in zip(got, run()):
+                assert torch.equal(a, b), now
